@@ -33,6 +33,7 @@ extern "C" {
 #define IQ_Q4_K 12
 #define IQ_Q5_K 13
 #define IQ_Q6_K 14
+#define IQ_I8 24
 #define IQ_BF16 30
 
 /* Where a caller-supplied buffer lives. */
@@ -314,6 +315,96 @@ int iq_state_set_profiling(iq_state* s, int on);
 /* Kernels this state has launched so far (graph replays included). */
 int iq_state_launch_count(const iq_state* s, int64_t* count);
 int iq_state_profile(const iq_state* s, char* buf, int len);
+
+/* ------------------------------------------------------------------ */
+/* Operator level: a paged key/value cache and the attention over it.  */
+/* (No reference counterpart: its cache is one f32 row list per        */
+/* sequence, src/qwen/quantized_attention.rs:409-507.)                 */
+/* ------------------------------------------------------------------ */
+/* One layer's cache: `pages` pages of `page_tokens` tokens (16, 32, 64, 128
+ * or 256) of `kv_heads` heads of `head_dim` (64, 128 or 256) elements, on the
+ * device that is current at creation.  Sequences name their pages in block
+ * tables that the caller owns, so that they grow by pages and share them.
+ * Per token and head one vector of keys and one of values, each in
+ *   IQ_I8   one byte an element: q = the integer nearest to 127 x / amax (ties
+ *           to even), value q * scale, scale = amax / 127 in f32;
+ *   IQ_F16  x / 2^e rounded to f16, value f16 * 2^e, 2^e per vector such that
+ *           amax / 2^e lies in [2^14, 2^15): no overflow at any magnitude.
+ * A vector that holds a NaN or an infinity reads back as NaN throughout. */
+typedef struct iq_kv iq_kv;
+
+/* Rows of several sequences.  Sequence s owns rows row_start[s] up to
+ * row_start[s + 1] - 1 (ascending; rows behind the last sequence belong to
+ * none and stay as they were); its row i stands at position[s] + i.  Page j
+ * of sequence s is table[s * table_ld + j]; a position >= 0 must lie inside
+ * the table's table_cols pages.  A negative position is padding.  table,
+ * position and row_start are device memory, read when the work runs;
+ * row_start may be NULL for one sequence that owns all rows.  max_rows: the
+ * most rows of one sequence, as far as the host knows (0: `rows`); it picks
+ * the kernel, and a wrong value costs time only. */
+typedef struct iq_kv_batch {
+  const int32_t* table;
+  const int32_t* position;
+  const int32_t* row_start;
+  int64_t table_ld;
+  int32_t table_cols;
+  int32_t seqs;
+  int32_t rows;
+  int32_t max_rows;
+} iq_kv_batch;
+
+/* Errors as elsewhere; what only the device can see (a position outside the
+ * table, a page id outside the pool) skips the row or token and is reported
+ * by iq_kv_status.  Calls are enqueued on `stream` (NULL: the legacy stream)
+ * of the cache's device, may be captured, and allocate nothing. */
+int iq_kv_create(int format, int kv_heads, int head_dim, int page_tokens, int64_t pages, iq_kv** out);
+/* (No call on the cache may still be running.) */
+void iq_kv_destroy(iq_kv* c);
+/* Device bytes of the pool, scales included. */
+int iq_kv_bytes(const iq_kv* c, int64_t* bytes);
+
+/* Quantise rows [row][kv_head][head_dim] of keys and values (dtype IQ_F32,
+ * IQ_F16 or IQ_BF16; strides in elements, elements of a head contiguous) into
+ * the cache.  Rows of one call must have positions of their own. */
+int iq_kv_append(iq_kv* c, const iq_kv_batch* b, int dtype, const void* k, int64_t k_row, int64_t k_head,
+                 const void* v, int64_t v_row, int64_t v_head, void* stream);
+/* The reverse: the values that the cache holds at the rows' positions, in
+ * `dtype`; rows at negative positions are zeros. */
+int iq_kv_read(const iq_kv* c, const iq_kv_batch* b, int dtype, void* k, int64_t k_row, int64_t k_head, void* v,
+               int64_t v_row, int64_t v_head, void* stream);
+
+/* Attention of new rows over the cache, which holds them already (append
+ * first).  Query head h reads KV head h / (heads / kv_heads).  The row at
+ * position p attends to the tokens t of its sequence with t <= p and, where
+ * window > 0, t > p - window or t < sinks; a row at a negative position sees
+ * nothing and is zeros.  Scores are scaled by `scale` (0: 1/sqrt(head_dim)).
+ * dtype (of q and out): IQ_F32, IQ_F16 or IQ_BF16; scores, softmax and sums
+ * are f32, f32 queries and weights enter the matrix instructions as two f16
+ * parts each, others rounded to f16 (a row's queries over a power of two, so
+ * that bf16's range is kept).
+ * chunk: tokens per split of a sequence (a multiple of 64), counted from
+ * position 0, whose partial results are joined in order; 0 lets the call
+ * choose by the batch's bounds.  With a chunk given and at most 64 query rows
+ * a sequence and KV head (max_rows * heads / kv_heads), a row's result
+ * depends on its own context and chunk only, bit for bit. */
+typedef struct iq_kv_attn {
+  int32_t dtype;
+  int32_t heads;
+  float scale;
+  int32_t window;
+  int32_t sinks;
+  int32_t chunk;
+} iq_kv_attn;
+/* Bytes of device workspace that iq_kv_attend needs for such a batch (its
+ * host fields only are read); 16-byte aligned, one for each call in flight. */
+int iq_kv_attend_workspace(const iq_kv* c, const iq_kv_batch* b, const iq_kv_attn* a, size_t* bytes);
+int iq_kv_attend(const iq_kv* c, const iq_kv_batch* b, const iq_kv_attn* a, const void* q, int64_t q_row,
+                 int64_t q_head, void* out, int64_t out_row, int64_t out_head, void* workspace, size_t workspace_bytes,
+                 void* stream);
+/* Synchronize `stream` and report (once) what calls on this cache met:
+ * IQ_EINVAL for a position or page id out of range, IQ_ETIMEDOUT when a
+ * bounded device wait gave up. */
+int iq_kv_status(iq_kv* c, void* stream);
 
 #ifdef __cplusplus
 }

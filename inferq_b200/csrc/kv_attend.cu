@@ -1,0 +1,655 @@
+// kv_attend.cu -- attention of few query rows over the paged cache (single
+// tokens, verify passes, any batch of short row groups), split over the
+// tokens, and the join of the splits.
+//
+// Mathematics.  For a query row at position p with scale c,
+//     s_t = c q . k_t,  o = sum_t 2^(s_t log2e - m) v_t / sum_t 2^(s_t log2e - m)
+// over the visible t, in one pass with the running maximum m and sum l.  Keys
+// and values are kept as k_t = a_t K_t, v_t = b_t V_t (K, V integers of 8
+// bits or f16, a and b f32), so the matrix instructions multiply K and V as
+// they are stored, a_t scales the score and b_t the weight:
+//     s_t = a_t (q . K_t),  o = sum_t (p_t b_t) V_t / l.
+// Weights enter as f16: p_t b_t 2^(14 - e), with 2^e above every b met so far
+// (e grows like m; the accumulators follow by powers of two), so the largest
+// weights are at most 2^14 and weights down to 2^-28 of them keep 11 bits.
+// f32 rows split queries and weights into two f16 parts each (22 bits).  A
+// query row is divided by a power of two first, which joins its scale.
+//
+// Work split.  A CTA takes 8 NT query rows (rows x heads of one KV head) and
+// one chunk of the tokens; partial results {m, l, o} go to the workspace and
+// a second kernel joins a row's chunks.  Keys are the M side of the first
+// product (S^T = K Q^T) and value elements that of the second (O^T = V^T
+// P^T), so 8 rows fill an instruction: with 8 query heads to a KV head a
+// single token needs no padding.  Four warps: a warp scores 16 of the tile's
+// 64 tokens for all rows, then sums a quarter of the head's elements over all
+// 64 tokens; so each stored byte is expanded to f16 once.  A fifth warp keeps
+// the next tiles' bulk copies in flight.  All rows' arithmetic is their own
+// and does not depend on NT: a row's result is the same in any batch.
+//
+// Bound: the cache's bytes for 8 rows, the tensor pipe and shared memory from
+// about 64 rows on.
+#include <cfloat>
+#include <climits>
+#include <type_traits>
+#include "kv_device.cuh"
+#include "kv_split.cuh"
+#include "model_kernels.cuh"
+
+namespace iq {
+namespace {
+
+using namespace kvp;
+
+constexpr int kTile = kKvTile;
+constexpr int kWarps = 4;
+constexpr int kWaitLimit = 1 << 20;
+constexpr int kDrainLimit = 1 << 24;  // for copies already in flight: none may outlive the CTA
+
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+// Transpose of an 8 x 8 matrix of f16 held as fragments.
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void consumers_sync() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
+// The same, and whether any thread's `bad` is set.
+__device__ __forceinline__ bool consumers_any(bool bad) {
+  uint32_t r;
+  asm volatile(
+      "{ .reg .pred p, q; setp.ne.u32 q, %1, 0; barrier.cta.red.or.pred p, 1, 128, q; selp.u32 %0, 1, 0, p; }"
+      : "=r"(r)
+      : "r"((uint32_t)bad)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack2(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+
+template <int HD, int FMT, int NT, bool F32Q>
+struct Geo {
+  static constexpr int kElt = FMT == kKvI8 ? 1 : 2;
+  static constexpr int kTileBytes = kTile * HD * kElt;  // of keys, and of values
+  static constexpr int kTQ = 8 * NT;
+  static constexpr int kQld = HD * 2 + 16;              // bytes of a staged query row
+  static constexpr int kQBytes = kTQ * kQld * (F32Q ? 2 : 1);
+  static constexpr int kPBytes = NT * 4 * 32 * 8 * (F32Q ? 2 : 1);
+  static constexpr int kFixed = kQBytes + kPBytes + 4 * kTQ * 4 + 2 * kTQ * 4 + 64;
+  // Stages: two CTAs on an SM where a stage is at most 32 KB, up to four
+  // stages of small tiles; a stage's 512 bytes of scales are counted in.
+  static constexpr int kPer = 2 * kTileBytes + 512;
+  static constexpr int kRoom = (2 * kTileBytes <= 32768 && kFixed <= 48 * 1024 ? 112 : 226) * 1024 - 2048 - kFixed;
+  static constexpr int kStages = kRoom / kPer > 4 ? 4 : kRoom / kPer;
+  static constexpr int kSmem = kStages * kPer + kFixed + 1024;
+  static_assert(kStages >= 2, "two stages keep a copy in flight");
+};
+
+template <int HD, int FMT, int NT, bool F32Q>
+__global__ void __launch_bounds__(160) kv_attend_kernel(const __grid_constant__ KvAttnArgs a, const bool vec) {
+  using G_ = Geo<HD, FMT, NT, F32Q>;
+  constexpr int TQ = G_::kTQ, ST = G_::kStages, QLD = G_::kQld;
+  __shared__ __align__(8) uint64_t full[ST], empty[ST];
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (su32(smem_raw) & 1023)) & 1023);
+  float* scales = reinterpret_cast<float*>(smem + ST * 2 * G_::kTileBytes);  // [stage][keys, values][64]
+  uint8_t* qs = reinterpret_cast<uint8_t*>(scales + ST * 128);               // [part][TQ][QLD]
+  uint2* ps = reinterpret_cast<uint2*>(qs + G_::kQBytes);                    // [part][NT][4][32]
+  float* mx = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(ps) + G_::kPBytes);  // [4][TQ]
+  float* cq = mx + 4 * TQ;                                                   // [TQ] row factor
+  int* rpos = reinterpret_cast<int*>(cq + TQ);                               // [TQ] row position, -1: none
+  int* evw = rpos + TQ;                                                      // [4]
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const KvPool& p = a.pool;
+  const int group = a.heads / p.nkv;
+  const int slot = blockIdx.x % a.slots;
+  const int kvh = blockIdx.x / a.slots % p.nkv;
+  const int tile = blockIdx.x / a.slots / p.nkv;
+  KvTileRows tr;
+  if (!kv_tile_rows(a.b, tile, TQ, group, lane, &tr)) return;
+  const KvSpan sp = kv_span(a, tr, TQ, slot);
+  if (sp.outside && threadIdx.x == 0) atomicOr(p.flag, kKvBadPage);
+  // splits that no row of the tile sees are not read by the join
+  if (sp.first >= sp.end && a.slots > 1) return;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ST; s++) {
+      bar_init(&full[s], 1);
+      bar_init(&empty[s], kWarps);
+    }
+    bar_init_fence();
+  }
+  __syncthreads();
+
+  if (warp == kWarps) {
+    // ------------------------------------------------------ copies in flight
+    const int rt = min(p.page_tokens, kTile), runs = kTile / rt;
+    const int64_t hb = kv_head_bytes(FMT, HD, p.page_tokens);
+    constexpr int kParts = FMT == kKvI8 ? 1 : HD / 64;  // contiguous pieces of a run
+    const int per = 2 * kParts + 2, copies = runs * per;
+    auto page_of = [&](int ti) {
+      // runs behind the last token are filled from the tile's first page
+      const int64_t pos = (int64_t)ti * kTile + (int64_t)lane * rt;
+      const bool in = lane < runs && pos < sp.tokens;
+      int page = in ? kv_page(p, a.b, tr.seq, pos) : -1;
+      const int first = __shfl_sync(0xffffffffu, page, 0);
+      if (!in) page = first;
+      return max(page, 0);
+    };
+    int it = 0, page = sp.first < sp.end ? page_of(sp.first) : 0;
+    bool ok = true;
+    for (int ti = sp.first; ti < sp.end; it++) {
+      const int s = it % ST;
+      if (it >= ST && !__all_sync(0xffffffffu, bar_wait(&empty[s], ((it / ST) + 1) & 1, kWaitLimit))) {
+        ok = false;
+        break;
+      }
+      if (lane == 0) bar_expect(&full[s], 2 * G_::kTileBytes + 2 * kTile * 4);
+      __syncwarp();
+      const int tp = (ti * kTile) & (p.page_tokens - 1);
+      uint8_t* kt = smem + s * 2 * G_::kTileBytes;
+      for (int c0 = 0; c0 < copies; c0 += 32) {
+        const int c = c0 + lane, run = min(c / per, runs - 1), what = c % per;
+        const int64_t at = (int64_t)__shfl_sync(0xffffffffu, page, run) * p.nkv + kvh;
+        if (c >= copies) continue;
+        if (what < 2 * kParts) {
+          const int part = what % kParts, isv = what / kParts;
+          const uint8_t* src = (isv ? p.v : p.k) + at * hb;
+          uint8_t* dst = kt + isv * G_::kTileBytes;
+          if constexpr (FMT == kKvI8)
+            bulk_load(su32(dst + run * rt * HD), src + (int64_t)tp * HD, rt * HD, &full[s]);
+          else
+            bulk_load(su32(dst + (part * kTile + run * rt) * 128), src + ((int64_t)part * p.page_tokens + tp) * 128,
+                      rt * 128, &full[s]);
+        } else {
+          const int isv = what - 2 * kParts;
+          bulk_load(su32(scales + s * 128 + isv * 64 + run * rt), (isv ? p.vs : p.ks) + at * p.page_tokens + tp, rt * 4,
+                    &full[s]);
+        }
+      }
+      ti = sp.next(ti);
+      if (ti < sp.end) page = page_of(ti);
+    }
+    if (!ok && lane == 0) atomicOr(p.flag, kKvTimeout);
+    // no copy outlives the CTA, also when the readers gave up
+    for (int s = 0; s < ST; s++)
+      if (it > s) bar_wait(&full[s], ((it - 1 - s) / ST) & 1, kDrainLimit);
+    return;
+  }
+
+  // ---------------------------------------------------------- query rows
+  // Elements are stored in the order in which a lane's fragments take them:
+  // 16 contiguous halves serve four instructions.
+  for (int r = warp; r < TQ; r += kWarps) {
+    const int rr = tr.r0 + r;
+    const bool live = rr < tr.nr;
+    const int i = rr / group, h = kvh * group + rr % group;
+    constexpr int N = HD / 32;
+    float x[N];
+    if (live) {
+      const int64_t o = (int64_t)(tr.row0 + i) * a.q.row + (int64_t)h * a.q.head + lane * N;
+      if constexpr (F32Q) load_n<float, N>(static_cast<const float*>(a.q.p) + o, vec, x);
+      else if (a.dtype == F16) load_n<__half, N>(static_cast<const __half*>(a.q.p) + o, vec, x);
+      else load_n<__nv_bfloat16, N>(static_cast<const __nv_bfloat16*>(a.q.p) + o, vec, x);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; j++) x[j] = 0.f;
+    }
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < N; j++) m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);
+    const int e = f16_exponent(__uint_as_float(__reduce_max_sync(0xffffffffu, m)));
+    const float f = pow2i(-e);
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+      const int d = lane * N + j;
+      const int o = FMT == kKvI8 ? d
+                                 : (d & ~63) + 16 * ((d & 7) >> 1) + 4 * ((d & 63) >> 4) + 2 * ((d >> 3) & 1) + (d & 1);
+      const float y = x[j] * f;
+      const __half hi = __float2half_rn(y);
+      *reinterpret_cast<__half*>(qs + r * QLD + 2 * o) = hi;
+      if constexpr (F32Q)
+        *reinterpret_cast<__half*>(qs + (TQ + r) * QLD + 2 * o) = __float2half_rn(y - __half2float(hi));
+    }
+    if (lane == 0) {
+      cq[r] = pow2i(e) * a.scale_log2e;
+      rpos[r] = live ? (int)max(min(tr.pos + i, (int64_t)INT_MAX), (int64_t)-1) : -1;
+    }
+  }
+  consumers_sync();
+
+  const int g = lane >> 2, t = lane & 3;
+  constexpr int kBlocks = HD / 32;                       // 32-element blocks of the head
+  constexpr int kMine = kBlocks >= kWarps ? kBlocks / kWarps : 1;
+  const bool sums = kBlocks >= kWarps || warp < kBlocks;  // hd 64: two warps sum
+  float o[kMine][2][NT][4];
+#pragma unroll
+  for (int b = 0; b < kMine; b++)
+#pragma unroll
+    for (int m = 0; m < 2; m++)
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) o[b][m][n][c] = 0.f;
+  float mrow[NT][2], l[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; n++) mrow[n][0] = mrow[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.f;
+  int ev = -100;  // so that 2^(14 - ev) is finite
+  bool failed = false;
+
+  int it = 0;
+  for (int ti = sp.first; ti < sp.end; ti = sp.next(ti), it++) {
+    const int s = it % ST, t0 = ti * kTile;
+    const uint32_t kt = su32(smem + s * 2 * G_::kTileBytes), vt = kt + G_::kTileBytes;
+    const float* sc = scales + s * 128;
+    const bool ok = __all_sync(0xffffffffu, bar_wait(&full[s], (it / ST) & 1, kWaitLimit));
+    float sa[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; n++) sa[n][0] = sa[n][1] = sa[n][2] = sa[n][3] = 0.f;
+    if (ok) {
+      // ------------------------------------------------ S^T = K Q^T
+      const uint32_t qa = su32(qs) + g * QLD + 32 * t;
+#pragma unroll
+      for (int j = 0; j < HD / 64; j++) {
+        uint32_t ka[4][4];  // fragments of the group's four instructions
+        if constexpr (FMT == kKvI8) {
+          const uint32_t at = kt + (16 * warp + g) * HD + (((4 * j + t) ^ i8_swizzle(g, HD)) << 4);
+          const uint4 w0 = lds128(at), w1 = lds128(at + 8 * HD);
+          const uint32_t u0[4] = {w0.x, w0.y, w0.z, w0.w}, u1[4] = {w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const uint2 x = biased4_to_f16(u0[i]), y = biased4_to_f16(u1[i]);
+            ka[i][0] = x.x, ka[i][1] = y.x, ka[i][2] = x.y, ka[i][3] = y.y;
+          }
+        } else {
+          const int m = lane >> 3, row = 16 * warp + (lane & 7) + (m & 1) * 8;
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            ldsm4(ka[i], kt + (j * kTile + row) * 128 + (((2 * i + (m >> 1)) ^ (row & 7)) << 4));
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+#pragma unroll
+          for (int part = 0; part < (F32Q ? 2 : 1); part++) {
+            const uint32_t at = qa + (part * TQ + n * 8) * QLD + 128 * j;
+            const uint4 q0 = lds128(at), q1 = lds128(at + 16);
+            mma16816(sa[n], ka[0][0], ka[0][1], ka[0][2], ka[0][3], q0.x, q0.y);
+            mma16816(sa[n], ka[1][0], ka[1][1], ka[1][2], ka[1][3], q0.z, q0.w);
+            mma16816(sa[n], ka[2][0], ka[2][1], ka[2][2], ka[2][3], q1.x, q1.y);
+            mma16816(sa[n], ka[3][0], ka[3][1], ka[3][2], ka[3][3], q1.z, q1.w);
+          }
+        }
+      }
+      // ------------------------------------- scores, masks, tile maxima
+      const int ta = t0 + 16 * warp + g;
+      const float k0 = sc[16 * warp + g], k1 = sc[16 * warp + g + 8];
+      const bool whole = sp.whole(t0, kTile);
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const int q = n * 8 + 2 * t + e;
+          const float f = cq[q];
+          float s0 = sa[n][e] * (k0 * f), s1 = sa[n][2 + e] * (k1 * f);
+          if (!whole) {
+            const int rp = rpos[q];
+            if (!sp.sees(rp, ta)) s0 = -INFINITY;
+            if (!sp.sees(rp, ta + 8)) s1 = -INFINITY;
+          }
+          sa[n][e] = s0;
+          sa[n][2 + e] = s1;
+          float m = fmaxf(s0, s1);
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+          if (lane < 4) mx[warp * TQ + q] = m;
+        }
+      // exponent above the tile's value scales
+      uint32_t vb = 0;
+      if (lane < 16 && t0 + 16 * warp + lane < sp.tokens) vb = __float_as_uint(sc[64 + 16 * warp + lane]);
+      if (vb >= 0x7f800000u) vb = 0;  // a NaN scale's rows are NaN whatever the exponent
+      vb = __reduce_max_sync(0xffffffffu, vb);
+      if (lane == 0) evw[warp] = max((int)(vb >> 23), 1) - 126;
+    }
+    if (consumers_any(!ok)) {
+      failed = true;
+      break;
+    }
+    // -------------------------------------------------- weights and sums
+    const int evn = max(max(ev, max(evw[0], evw[1])), max(evw[2], evw[3]));
+    const float shrink = ev - evn < -126 ? 0.f : pow2i(ev - evn);
+    const float up = pow2i(-evn) * 16384.f;
+    ev = evn;
+    const float v0 = sc[64 + 16 * warp + g] * up, v1 = sc[64 + 16 * warp + g + 8] * up;
+    float fo[NT][2];
+    bool moved = false;
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+      float w[4];
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const int q = n * 8 + 2 * t + e;
+        const float m = fmaxf(fmaxf(mrow[n][e], fmaxf(mx[q], mx[TQ + q])), fmaxf(mx[2 * TQ + q], mx[3 * TQ + q]));
+        const float ms = m == -INFINITY ? 0.f : m;
+        const float alpha = ex2(mrow[n][e] - ms);
+        mrow[n][e] = m;
+        const float p0 = ex2(sa[n][e] - ms), p1 = ex2(sa[n][2 + e] - ms);
+        l[n][e] = l[n][e] * alpha + (p0 + p1);
+        fo[n][e] = alpha * shrink;
+        moved |= fo[n][e] != 1.f;
+        // a hidden token weighs zero whatever its scale is
+        w[e] = sa[n][e] == -INFINITY ? 0.f : p0 * v0;
+        w[2 + e] = sa[n][2 + e] == -INFINITY ? 0.f : p1 * v1;
+      }
+      const uint32_t h0 = pack2(w[0], w[1]), h1 = pack2(w[2], w[3]);
+      ps[(n * 4 + warp) * 32 + lane] = make_uint2(transpose8(h0), transpose8(h1));
+      if constexpr (F32Q) {
+        const float2 f0 = unpack2(h0), f1 = unpack2(h1);
+        ps[((NT + n) * 4 + warp) * 32 + lane] =
+            make_uint2(transpose8(pack2(w[0] - f0.x, w[1] - f0.y)), transpose8(pack2(w[2] - f1.x, w[3] - f1.y)));
+      }
+    }
+    consumers_sync();
+    // --------------------------------------------------- O^T += V^T P^T
+    if (sums) {
+      if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int b = 0; b < kMine; b++)
+#pragma unroll
+          for (int m = 0; m < 2; m++)
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+              o[b][m][n][0] *= fo[n][0];
+              o[b][m][n][1] *= fo[n][1];
+              o[b][m][n][2] *= fo[n][0];
+              o[b][m][n][3] *= fo[n][1];
+            }
+      }
+#pragma unroll
+      for (int kk = 0; kk < 4; kk++) {
+        uint32_t va[kMine][2][4];
+#pragma unroll
+        for (int b = 0; b < kMine; b++) {
+          const int blk = warp * kMine + b;
+          if constexpr (FMT == kKvI8) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const int tok = 16 * kk + 2 * t + (i & 1) + 8 * (i >> 1);
+              w[i] = lds32(vt + tok * HD + (((2 * blk + (g >> 2)) ^ i8_swizzle(tok, HD)) << 4) + ((4 * g) & 15));
+            }
+            // bytes of two tokens side by side, element by element
+            const uint2 x0 = biased4_to_f16(__byte_perm(w[0], w[1], 0x5140)),
+                        x1 = biased4_to_f16(__byte_perm(w[0], w[1], 0x7362)),
+                        y0 = biased4_to_f16(__byte_perm(w[2], w[3], 0x5140)),
+                        y1 = biased4_to_f16(__byte_perm(w[2], w[3], 0x7362));
+            va[b][0][0] = x0.x, va[b][0][1] = x0.y, va[b][0][2] = y0.x, va[b][0][3] = y0.y;
+            va[b][1][0] = x1.x, va[b][1][1] = x1.y, va[b][1][2] = y1.x, va[b][1][3] = y1.y;
+          } else {
+            const int m = lane >> 3, tok = 16 * kk + (lane & 7) + (m >> 1) * 8;
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++) {
+              const int c = blk * 4 + mt * 2 + (m & 1);
+              ldsm4t(va[b][mt], vt + ((c >> 3) * kTile + tok) * 128 + (((c & 7) ^ (tok & 7)) << 4));
+            }
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int part = 0; part < (F32Q ? 2 : 1); part++) {
+            const uint2 w = ps[((part * NT + n) * 4 + kk) * 32 + lane];
+#pragma unroll
+            for (int b = 0; b < kMine; b++)
+#pragma unroll
+              for (int mt = 0; mt < 2; mt++)
+                mma16816(o[b][mt][n], va[b][mt][0], va[b][mt][1], va[b][mt][2], va[b][mt][3], w.x, w.y);
+          }
+      }
+    }
+    __syncwarp();
+    if (lane == 0) bar_arrive(&empty[s]);
+  }
+  if (failed) {
+    if (threadIdx.x == 0) atomicOr(p.flag, kKvTimeout);
+    return;
+  }
+  // ------------------------------------------------------------- results
+  consumers_sync();  // mx is read no more
+#pragma unroll
+  for (int n = 0; n < NT; n++)
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      float v = l[n][e];
+      v += __shfl_xor_sync(0xffffffffu, v, 4);
+      v += __shfl_xor_sync(0xffffffffu, v, 8);
+      v += __shfl_xor_sync(0xffffffffu, v, 16);
+      if (lane < 4) mx[warp * TQ + n * 8 + 2 * t + e] = v;
+    }
+  consumers_sync();
+  const float back = pow2i(ev);
+#pragma unroll
+  for (int n = 0; n < NT; n++)
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      const int q = n * 8 + 2 * t + e, rr = tr.r0 + q;
+      if (rr >= tr.nr) continue;
+      const float sum = (mx[q] + mx[TQ + q]) + (mx[2 * TQ + q] + mx[3 * TQ + q]);
+      const int row = tr.row0 + rr / group, h = kvh * group + rr % group;
+      const int64_t rh = (int64_t)row * a.heads + h;
+      const float f = a.slots > 1 ? 0x1p-14f : sum != 0.f ? __fdiv_rn(0x1p-14f, sum) : 0.f;
+      if (a.slots > 1 && warp == 0 && g == 0) a.ml[rh * a.slots + slot] = make_float2(mrow[n][e], sum);
+      if (!sums) continue;
+#pragma unroll
+      for (int b = 0; b < kMine; b++) {
+        const int blk = warp * kMine + b;
+        // i8: elements 4g .. 4g+3 of the block; f16: g, g+8, g+16, g+24
+        const float x[4] = {o[b][0][n][e] * back * f, o[b][0][n][2 + e] * back * f, o[b][1][n][e] * back * f,
+                            o[b][1][n][2 + e] * back * f};
+        auto put = [&](auto* dst, bool v4) {
+          using T = std::remove_reference_t<decltype(*dst)>;
+          if constexpr (FMT == kKvI8) {
+            store_n<T, 4>(dst + blk * 32 + 4 * g, v4, x);
+          } else {
+#pragma unroll
+            for (int c = 0; c < 4; c++) dst[blk * 32 + g + 8 * c] = from_f<T>(x[c]);
+          }
+        };
+        if (a.slots > 1) {
+          put(a.part + (rh * a.slots + slot) * HD, true);
+        } else {
+          const int64_t at = (int64_t)row * a.out.row + (int64_t)h * a.out.head;
+          if constexpr (F32Q) put(static_cast<float*>(a.out.p) + at, vec);
+          else if (a.dtype == F16) put(static_cast<__half*>(a.out.p) + at, vec);
+          else put(static_cast<__nv_bfloat16*>(a.out.p) + at, vec);
+        }
+      }
+    }
+}
+
+// A row's splits joined: out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c
+// over the chunks c that the row sees.  One CTA per (row, head); chunk c goes
+// to thread group c mod NG, whose sums are joined in order, so the result
+// depends on the row's own chunks only.
+template <class T, int HD>
+__global__ void __launch_bounds__(256) kv_join_kernel(const __grid_constant__ KvAttnArgs a, const int tq,
+                                                      const bool vec) {
+  constexpr int TPG = HD / 4, NG = 256 / TPG, kWeights = 1024;
+  __shared__ float wt[kWeights], red[8], sums[NG];
+  __shared__ float4 os[NG][TPG];
+  pdl_wait();
+  const int row = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
+  const int lane = threadIdx.x & 31, grp = threadIdx.x / TPG, d4 = threadIdx.x % TPG;
+  int i;
+  const int seq = kv_seq_of_row(a.b, row, lane, &i);
+  if (seq < 0) return;
+  const int group = a.heads / a.pool.nkv;
+  const int64_t base = a.b.position[seq], pos = base + i;
+  const int tile0 = (i * group + h % group) / tq * tq;  // the row's tile begins here
+  const KvChunks ch = kv_chunks(a, base + tile0 / group);
+  const KvRowChunks rc = kv_row_chunks(a, ch, pos);
+  const int64_t rh = (int64_t)row * a.heads + h;
+  const float2* ml = a.ml + rh * a.slots;
+  const float* part = a.part + rh * a.slots * HD + 4 * d4;
+  float mxv = -INFINITY;
+  for (int c = threadIdx.x; c < rc.count; c += 256) mxv = fmaxf(mxv, ml[ch.slot(rc.chunk(c))].x);
+#pragma unroll
+  for (int w = 16; w; w >>= 1) mxv = fmaxf(mxv, __shfl_xor_sync(0xffffffffu, mxv, w));
+  if (lane == 0) red[threadIdx.x >> 5] = mxv;
+  __syncthreads();
+  float M = red[0];
+#pragma unroll
+  for (int w = 1; w < 8; w++) M = fmaxf(M, red[w]);
+  const float ms = M == -INFINITY ? 0.f : M;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+  for (int c0 = 0; c0 < rc.count; c0 += kWeights) {
+    const int nc = min(kWeights, rc.count - c0);
+    __syncthreads();
+    for (int c = threadIdx.x; c < nc; c += 256) wt[c] = kvp::ex2(ml[ch.slot(rc.chunk(c0 + c))].x - ms);
+    __syncthreads();
+    // the group's chunks: those with chunk index = grp mod NG, in order
+    for (int r = 0; r < 2; r++) {
+      // the always-visible chunks, then the window's
+      const int lo = max(c0, r ? rc.firsts : 0), hi = min(c0 + nc, r ? rc.count : rc.firsts);
+      if (lo >= hi) continue;
+      const int first = rc.chunk(lo);
+#pragma unroll 4
+      for (int c = lo + ((grp - first % NG + NG) % NG); c < hi; c += NG) {
+        const int sl = ch.slot(rc.chunk(c));
+        const float w = wt[c - c0];
+        const float4 x = *reinterpret_cast<const float4*>(part + (int64_t)sl * HD);
+        acc.x = fmaf(w, x.x, acc.x);
+        acc.y = fmaf(w, x.y, acc.y);
+        acc.z = fmaf(w, x.z, acc.z);
+        acc.w = fmaf(w, x.w, acc.w);
+        sum = fmaf(w, ml[sl].y, sum);
+      }
+    }
+  }
+  os[grp][d4] = acc;
+  if (d4 == 0) sums[grp] = sum;
+  __syncthreads();
+  if (grp) return;
+  for (int k = 1; k < NG; k++) {
+    const float4 x = os[k][d4];
+    acc.x += x.x;
+    acc.y += x.y;
+    acc.z += x.z;
+    acc.w += x.w;
+    sum += sums[k];
+  }
+  const float f = sum != 0.f ? __fdiv_rn(1.f, sum) : 0.f;
+  const float x[4] = {acc.x * f, acc.y * f, acc.z * f, acc.w * f};
+  store_n<T, 4>(static_cast<T*>(a.out.p) + (int64_t)row * a.out.row + (int64_t)h * a.out.head + 4 * d4, vec, x);
+}
+
+template <int HD, int FMT, int NT, bool F32Q>
+cudaError_t launch_split(const KvAttnArgs& a, int64_t ctas, bool vec, cudaStream_t st) {
+  using G_ = Geo<HD, FMT, NT, F32Q>;
+  static bool configured[64] = {};
+  static std::mutex mu;
+  const cudaError_t e = once_per_device(configured, mu, [] {
+    return cudaFuncSetAttribute(kv_attend_kernel<HD, FMT, NT, F32Q>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                G_::kSmem);
+  });
+  if (e != cudaSuccess) return e;
+  kv_attend_kernel<HD, FMT, NT, F32Q><<<(unsigned)ctas, 160, G_::kSmem, st>>>(a, vec);
+  return cudaGetLastError();
+}
+
+bool strides_ok(const KvTensor& t, int item, int bytes) {
+  return ((uintptr_t)t.p | (uintptr_t)(t.row * item) | (uintptr_t)(t.head * item)) % bytes == 0;
+}
+
+template <class T, int HD>
+cudaError_t launch_join(const KvAttnArgs& a, int tq, cudaStream_t st) {
+  return launch_pdl(kv_join_kernel<T, HD>, dim3((unsigned)((int64_t)a.b.rows * a.heads)), dim3(256), 0, st, true, a, tq,
+                    strides_ok(a.out, sizeof(T), 4 * sizeof(T)));
+}
+
+}  // namespace
+
+size_t kv_attend_plan(KvAttnArgs& a, int max_rows) { return kv_plan(a, max_rows); }
+
+void kv_attend_bind(KvAttnArgs& a, void* workspace) {
+  if (a.slots == 1) return;
+  a.part = static_cast<float*>(workspace);
+  a.ml = reinterpret_cast<float2*>(a.part + (int64_t)a.b.rows * a.heads * a.slots * a.pool.hd);
+}
+
+cudaError_t kv_attend_launch(const KvAttnArgs& a, int max_rows, cudaStream_t st) {
+  const int tq = kv_tile_query_rows(a, max_rows);
+  const int64_t ctas = kv_tiles_bound(a, tq) * a.pool.nkv * a.slots;
+  if (ctas >= (1ll << 31)) return cudaErrorInvalidValue;
+  const int item = a.dtype == F32 ? 4 : 2;
+  // one flag for reading queries (hd / 32 elements a lane) and writing four
+  // elements: both are whole words of up to 16 bytes
+  const bool vec = strides_ok(a.q, item, 16) && strides_ok(a.out, item, 16);
+  auto by_rows = [&](auto hd, auto fmt, auto f32) {
+    constexpr int HD = decltype(hd)::value, FMT = decltype(fmt)::value;
+    constexpr bool F = decltype(f32)::value;
+    switch (tq) {
+      case 8: return launch_split<HD, FMT, 1, F>(a, ctas, vec, st);
+      case 16: return launch_split<HD, FMT, 2, F>(a, ctas, vec, st);
+      case 32: return launch_split<HD, FMT, 4, F>(a, ctas, vec, st);
+      default: return launch_split<HD, FMT, 8, F>(a, ctas, vec, st);
+    }
+  };
+  auto by_type = [&](auto hd, auto fmt) {
+    return a.dtype == F32 ? by_rows(hd, fmt, std::true_type()) : by_rows(hd, fmt, std::false_type());
+  };
+  auto by_format = [&](auto hd) {
+    return a.pool.format == kKvI8 ? by_type(hd, std::integral_constant<int, kKvI8>())
+                                  : by_type(hd, std::integral_constant<int, kKvF16>());
+  };
+  auto join = [&](auto hd) {
+    constexpr int HD = decltype(hd)::value;
+    return a.dtype == F32   ? launch_join<float, HD>(a, tq, st)
+           : a.dtype == F16 ? launch_join<__half, HD>(a, tq, st)
+                            : launch_join<__nv_bfloat16, HD>(a, tq, st);
+  };
+  auto go = [&](auto hd) {
+    const cudaError_t e = by_format(hd);
+    return e != cudaSuccess || a.slots == 1 ? e : join(hd);
+  };
+  switch (a.pool.hd) {
+    case 64: return go(std::integral_constant<int, 64>());
+    case 128: return go(std::integral_constant<int, 128>());
+    case 256: return go(std::integral_constant<int, 256>());
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+}  // namespace iq

@@ -1,0 +1,185 @@
+// kv_split.cuh -- which query rows a CTA takes, which tokens they see, and
+// how the tokens are split into chunks.  The attention kernels and the join
+// of their partial results go by the same functions.
+//
+// Chunk c holds the positions [c * chunk, (c + 1) * chunk) of a sequence.  A
+// tile of query rows at positions pa..pb has partial results for the slots
+// 0 .. slots - 1: the chunks of the always-visible first tokens, then those
+// from the first token that the row at pa sees.
+#pragma once
+#include <algorithm>
+#include "kv_device.cuh"
+
+namespace iq {
+
+__host__ __device__ inline int64_t kv_min(int64_t a, int64_t b) { return a < b ? a : b; }
+__host__ __device__ inline int64_t kv_max(int64_t a, int64_t b) { return a > b ? a : b; }
+
+struct KvTileRows {
+  int seq, row0;  // the sequence and its first row
+  int r0, nr;     // first query row of the tile and query rows (row x head of the KV head) of the sequence
+  int64_t pos;    // position of the sequence's first row
+};
+
+// Tile `tile` of `tq` query rows, counted through the sequences; false when
+// the batch has fewer.  Warp-wide; every lane gets the result.
+__device__ __forceinline__ bool kv_tile_rows(const KvBatch& b, int tile, int tq, int group, int lane, KvTileRows* t) {
+  int n;
+  if (!b.row_start) {
+    t->seq = t->row0 = 0;
+    n = b.rows;
+    t->r0 = tile * tq;
+  } else if (group % tq == 0) {  // no tile crosses a row: no sum over sequences
+    const int per = group / tq, row = tile / per;
+    int i;
+    t->seq = row < b.rows ? kv_seq_of_row(b, row, lane, &i) : -1;
+    if (t->seq < 0) return false;
+    t->row0 = row - i;
+    n = b.row_start[t->seq + 1] - t->row0;
+    t->r0 = i * group + tile % per * tq;
+  } else {
+    int before = 0;  // tiles of the sequences up to s0
+    t->seq = -1;
+    for (int s0 = 0; s0 < b.seqs; s0 += 32) {
+      const int s = s0 + lane;
+      const int rows = s < b.seqs ? max(b.row_start[s + 1] - b.row_start[s], 0) : 0;
+      const int tiles = (int)(((int64_t)rows * group + tq - 1) / tq);
+      int sum = tiles;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += x;
+      }
+      const uint32_t past = __ballot_sync(0xffffffffu, before + sum > tile);
+      if (past) {
+        const int at = __ffs(past) - 1;
+        t->seq = s0 + at;
+        t->r0 = (tile - before - __shfl_sync(0xffffffffu, sum - tiles, at)) * tq;
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (t->seq < 0) return false;
+    t->row0 = b.row_start[t->seq];
+    n = b.row_start[t->seq + 1] - t->row0;
+  }
+  if (t->row0 < 0) return false;
+  t->nr = min(n, b.rows - t->row0) * group;
+  t->pos = b.position[t->seq];
+  return t->r0 < t->nr;
+}
+
+struct KvChunks {
+  int first_chunks;  // chunks of the always-visible first tokens
+  int window0;       // first chunk of the window part
+  __host__ __device__ int slot(int c) const { return c < first_chunks ? c : first_chunks + c - window0; }
+  __host__ __device__ int chunk(int s) const { return s < first_chunks ? s : window0 + s - first_chunks; }
+};
+// pa: position of the tile's first row.
+__host__ __device__ inline KvChunks kv_chunks(const KvAttnArgs& a, int64_t pa) {
+  KvChunks c = {0, 0};
+  if (a.window) {
+    c.first_chunks = (a.sinks + a.chunk - 1) / a.chunk;
+    c.window0 = (int)kv_max(c.first_chunks, kv_max(pa - a.window + 1, 0) / a.chunk);
+  }
+  return c;
+}
+
+// The chunks that hold a visible token of the row at `pos`, ascending.
+struct KvRowChunks {
+  int firsts, window0, count;
+  __host__ __device__ int chunk(int j) const { return j < firsts ? j : window0 + j - firsts; }
+};
+__host__ __device__ inline KvRowChunks kv_row_chunks(const KvAttnArgs& a, const KvChunks& ch, int64_t pos) {
+  const int64_t cap = (int64_t)a.b.table_cols << a.pool.page_shift;
+  const int64_t top = kv_min(pos, cap - 1);
+  if (top < 0) return {0, 0, 0};
+  KvRowChunks r;
+  const int last = (int)(top / a.chunk);
+  r.firsts = (int)kv_min(ch.first_chunks, last + 1);
+  r.window0 = a.window ? (int)kv_max(ch.first_chunks, kv_max(pos - a.window + 1, 0) / a.chunk) : 0;
+  r.count = r.firsts + (int)kv_max(last - r.window0 + 1, 0);
+  return r;
+}
+
+// The tokens of one chunk that a tile of rows sees, in tiles of 64.
+struct KvSpan {
+  int first, end;       // tiles first, next(first), ... below end
+  int tokens;           // tokens up to the last row's, as far as the table reaches
+  int pa, pb;           // first and last row's position
+  int window, sinks;
+  bool outside;         // a row stands behind the table
+  __host__ __device__ int skip(int ti) const {
+    if (window && ti * 64 >= sinks && ti * 64 + 63 <= pa - window) return (pa - window + 1) >> 6;
+    return ti;
+  }
+  __host__ __device__ int next(int ti) const { return skip(ti + 1); }
+  // Whether every row sees all tokens [t0, t0 + n).
+  __host__ __device__ bool whole(int t0, int n) const {
+    return t0 + n - 1 <= pa && t0 + n <= tokens && (!window || t0 > pb - window || t0 + n <= sinks);
+  }
+  // Whether the row at position rp (-1: none) sees token t.
+  __host__ __device__ bool sees(int rp, int t) const {
+    return t <= rp && t < tokens && (!window || t > rp - window || t < sinks);
+  }
+};
+__host__ __device__ inline KvSpan kv_span(const KvAttnArgs& a, const KvTileRows& t, int tq, int slot) {
+  const int group = a.heads / a.pool.nkv;
+  const int64_t cap = (int64_t)a.b.table_cols << a.pool.page_shift;
+  const int64_t pa = t.pos + t.r0 / group, pb = t.pos + (kv_min(t.r0 + tq, t.nr) - 1) / group;
+  const int64_t top = (1ll << 31) - 1;
+  KvSpan s;
+  s.pa = (int)kv_max(kv_min(pa, top), -top);
+  s.pb = (int)kv_max(kv_min(pb, top), -top);
+  s.outside = pb >= cap;
+  s.tokens = (int)kv_max(kv_min(pb + 1, cap), 0);
+  s.window = a.window;
+  s.sinks = a.sinks;
+  const int64_t c0 = (int64_t)kv_chunks(a, pa).chunk(slot) * a.chunk;
+  const int64_t c1 = kv_min(c0 + a.chunk, s.tokens);
+  s.first = s.skip((int)kv_min(c0 >> 6, 1 << 26));
+  s.end = (int)((c1 + 63) >> 6);
+  return s;
+}
+
+// ------------------------------------------------------------ host side
+constexpr int kKvTile = 64;  // tokens a tile
+
+// Query rows of a tile: the fewest of 8, 16, 32, 64 that take a sequence's
+// rows of one KV head at once.
+inline int kv_tile_query_rows(const KvAttnArgs& a, int max_rows) {
+  const int64_t r = (int64_t)(max_rows ? std::min(max_rows, a.b.rows) : a.b.rows) * (a.heads / a.pool.nkv);
+  return r <= 8 ? 8 : r <= 16 ? 16 : r <= 32 ? 32 : 64;
+}
+inline int64_t kv_tiles_bound(const KvAttnArgs& a, int tq) {
+  const int64_t r = (int64_t)a.b.rows * (a.heads / a.pool.nkv);
+  if (!a.b.row_start) return ceil_div(r, tq);
+  if ((a.heads / a.pool.nkv) % tq == 0) return r / tq;
+  return r / tq + std::min(a.b.seqs, a.b.rows);
+}
+
+
+// Fills chunk (where it is 0) and slots; the workspace bytes.
+inline size_t kv_plan(KvAttnArgs& a, int max_rows) {
+  const int group = a.heads / a.pool.nkv, tq = kv_tile_query_rows(a, max_rows);
+  const int64_t cap = (int64_t)a.b.table_cols * a.pool.page_tokens;
+  const int tile_tokens = (tq - 1) / group + 1;
+  const int64_t span = a.window ? std::min<int64_t>(cap, (int64_t)a.window + a.sinks + tile_tokens + kKvTile) : cap;
+  const int64_t items = kv_tiles_bound(a, tq) * a.pool.nkv;
+  if (!a.chunk) {
+    // Halve the split until two CTAs an SM have two chunks each to take, or a
+    // chunk is two tiles.
+    int64_t chunk = std::max<int64_t>(align_up(span, kKvTile), 2 * kKvTile);
+    while (chunk > 2 * kKvTile && items * ceil_div(span, chunk) < 4 * 148) chunk = align_up(chunk / 2, kKvTile);
+    a.chunk = (int)chunk;
+  }
+  const int64_t all = std::max<int64_t>(ceil_div(cap, a.chunk), 1);
+  a.slots = (int)all;
+  if (a.window)
+    a.slots = (int)std::min<int64_t>(all, ceil_div(a.sinks, a.chunk) + ((int64_t)a.window + tile_tokens) / a.chunk + 2);
+  if (a.slots == 1) return 0;
+  const int64_t parts = (int64_t)a.b.rows * a.heads * a.slots;
+  return (size_t)(parts * a.pool.hd * 4 + parts * 8);
+}
+
+}  // namespace iq
