@@ -33,6 +33,7 @@
 #include <type_traits>
 #include "kv_device.cuh"
 #include "kv_split.cuh"
+#include "kv_wide.h"
 #include "model_kernels.cuh"
 
 namespace iq {
@@ -641,7 +642,7 @@ cudaError_t kv_attend_launch(const KvAttnArgs& a, int max_rows, cudaStream_t st)
                             : launch_join<__nv_bfloat16, HD>(a, tq, st);
   };
   auto go = [&](auto hd) {
-    const cudaError_t e = by_format(hd);
+    const cudaError_t e = tq > 64 ? kv_attend_wide_launch(a, ctas, vec, st) : by_format(hd);
     return e != cudaSuccess || a.slots == 1 ? e : join(hd);
   };
   switch (a.pool.hd) {

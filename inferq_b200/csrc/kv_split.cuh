@@ -146,10 +146,10 @@ __host__ __device__ inline KvSpan kv_span(const KvAttnArgs& a, const KvTileRows&
 constexpr int kKvTile = 64;  // tokens a tile
 
 // Query rows of a tile: the fewest of 8, 16, 32, 64 that take a sequence's
-// rows of one KV head at once.
+// rows of one KV head at once; above 64 rows the tensor-core kernel's 128.
 inline int kv_tile_query_rows(const KvAttnArgs& a, int max_rows) {
   const int64_t r = (int64_t)(max_rows ? std::min(max_rows, a.b.rows) : a.b.rows) * (a.heads / a.pool.nkv);
-  return r <= 8 ? 8 : r <= 16 ? 16 : r <= 32 ? 32 : 64;
+  return r <= 8 ? 8 : r <= 16 ? 16 : r <= 32 ? 32 : r <= 64 ? 64 : 128;
 }
 inline int64_t kv_tiles_bound(const KvAttnArgs& a, int tq) {
   const int64_t r = (int64_t)a.b.rows * (a.heads / a.pool.nkv);
