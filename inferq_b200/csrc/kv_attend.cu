@@ -43,8 +43,8 @@ using namespace kvp;
 
 constexpr int kTile = kKvTile;
 constexpr int kWarps = 4;
-constexpr int kWaitLimit = 1 << 20;
-constexpr int kDrainLimit = 1 << 24;  // for copies already in flight: none may outlive the CTA
+constexpr int kWaitLimit = 1 << 19;   // of 2 us each: a second
+constexpr int kDrainLimit = 1 << 21;  // for copies already in flight: none may outlive the CTA
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {

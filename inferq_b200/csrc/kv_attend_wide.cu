@@ -13,22 +13,28 @@
 // tensor rate (128 bytes a cycle).  TMEM: O in hd columns, two buffers of S
 // (64 columns each; P replaces S in place), Q.  K tiles are K-major and V
 // tiles MN-major in the 128-byte swizzle, in which the f16 cache already
-// keeps its pages: its tiles arrive by bulk copies alone.  i8 tiles are
-// expanded to f16 integers on the way (two groups of four warps, one for keys
-// and one for values, global loads in flight while the other tile is written).
+// keeps its pages: its tiles arrive by bulk copies alone.  i8 tiles arrive as
+// bytes in small stages, and eight warps expand them to f16 integers.
 //
 // f32 rows enter as two f16 parts: Q's second part is a shared-memory operand
 // of a second product into the same S, P's second part lies beside the first.
 //
-// Softmax: four warps, one row a thread, so that no maximum crosses a lane.
-// The running maximum moves only when a tile exceeds it by more than 2^8 (the
-// accumulator is rescaled in TMEM then); weights are at most
-// 2^8 * 2^(7 - 2): ev keeps two binades of room above the first value scales.
-// The weight of the largest score is at least 2^-3 * 2^5, and f16 keeps 11
-// bits down to 2^-14, i.e. to 2^-16 of it, and absolute 2^-25 below.
+// Softmax: sixteen warps in two groups that take the tiles in turn, so that one
+// group's waits and exponentials lie beside the other's; a row's 64 scores lie
+// with two threads, 32 each.  All share the row's maximum: the group of tile i
+// decides on it (after the group of tile i - 1 has), and it moves only when a
+// tile exceeds it by more than 2^8 (one barrier a tile says whether any row of
+// a pair of warps needs that; the accumulator is then rescaled in TMEM).  With
+// m the maximum and ev two binades above the first value scales, a row's
+// reference is r = m - 7 + ev:
+//     p_t = 2^(s_t log2e - r),  weight p_t b_t <= 2^8 2^7 2^-ev b_t <= 2^15,
+// the weight of the largest score about 2^4, and f16 keeps 11 bits down to
+// 2^-14 and 2^-25 below.  {r, l, o} are the partial result.
 //
-// Warps: 0-3 softmax and results, 4 issues the MMAs, 5.. load (one warp of
-// bulk copies for f16, eight warps for i8).  Every wait is bounded; one that
+// Warps: 0-15 softmax and results, 16 issues the MMAs (one elected lane: issued
+// under a plain lane test each instruction cost four times the cycles), 17-20
+// request keys and values (two warps each, tiles in turn: a tile costs one some
+// 2000 cycles of dependent address arithmetic and waits), 21-28 expand i8.  Every wait is bounded; one that
 // runs out sets the cache's flag, and the CTA winds down (copies and MMAs
 // drained, TMEM freed) without results.
 #include <cfloat>
@@ -44,21 +50,27 @@ namespace {
 using namespace kvp;
 
 constexpr int kM = 128, kT = 64;
-constexpr int kWaitLimit = 1 << 20;
-constexpr int kDrainLimit = 1 << 24;
+constexpr int kWaitLimit = 1 << 19;  // of 2 us each: a second
+constexpr int kDrainLimit = 1 << 21;
 constexpr int kScaleRing = 4;
-constexpr int kMmaWarp = 4, kLoadWarp = 5;
+constexpr int kSoftWarps = 16, kMmaWarp = 16, kLoadWarp = 17, kExpandWarp = 21;
 
 template <int HD, int FMT, bool F32Q>
 struct Geo {
   static constexpr int kTileBytes = kT * HD * 2;  // an f16 tile of keys or values
   static constexpr int kQlo = F32Q ? kM * HD * 2 : 0;
-  // f32 rows at hd 256: 64 KB of Q parts and two tiles each; three otherwise
-  static constexpr int kRing = F32Q && HD == 256 ? 2 : HD == 256 ? 3 : 4;
-  static constexpr int kScaleBytes = kScaleRing * (2 * kT + 4) * 4;
-  static constexpr int kSmem = 2 * kRing * kTileBytes + kQlo + kScaleBytes + 1024;
-  static constexpr int kLoadWarps = FMT == kKvI8 ? 8 : 1;
-  static constexpr int kThreads = (kLoadWarp + kLoadWarps) * 32;
+  static constexpr int kRing = HD < 256 ? 4 : FMT == kKvI8 || F32Q ? 2 : 3;
+  // i8 tiles pass through stages of bytes, for keys and for values each: whole
+  // tiles, but for f32 rows at hd 256, whose second parts leave room for three
+  // quarters of one
+  static constexpr bool kSmall = F32Q && HD == 256;
+  static constexpr int kStageTokens = kSmall ? 16 : kT;
+  static constexpr int kStage = FMT == kKvI8 ? kStageTokens * HD : 0;
+  static constexpr int kStages = FMT != kKvI8 ? 1 : kSmall || HD < 256 ? 3 : 2;
+  static constexpr int kScaleBytes = kScaleRing * (2 * kT + 4) * 4 + 6 * kM * 4;
+  static constexpr int kSmem = 2 * kRing * kTileBytes + kQlo + 2 * kStages * kStage + kScaleBytes + 1024;
+  static constexpr int kExpandWarps = FMT == kKvI8 ? 8 : 0;
+  static constexpr int kThreads = (kExpandWarp + kExpandWarps) * 32;
   static constexpr uint32_t kTmemS = HD, kTmemQ = HD + 2 * kT;
   static constexpr uint32_t kTmemCols = HD + 2 * kT + HD / 2 > 256 ? 512 : 256;
   static_assert(HD + 2 * kT + HD / 2 <= 512, "O, S and Q fit the tensor memory");
@@ -120,17 +132,71 @@ __device__ __forceinline__ void tmem_wait(uint32_t (&v)[32]) {
                :
                : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t a, const uint32_t (&v)[32]) {
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void tmem_st16(uint32_t a, const uint32_t (&v)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
-      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(a),
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(a),
       "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
-      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
-      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
-__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st8(uint32_t a, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(a), "r"(v[0]), "r"(v[1]),
+               "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t a, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(a)
+      : "memory");
+}
+// Two f32 in one operation (sm_100's packed forms, each lane rounded as the
+// scalar operation).
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{ .reg .b64 x, y; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mul.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x; }"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{ .reg .b64 x, y; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; add.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x; }"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mov.b64 z, {%6, %7};\n"
+      "fma.rn.f32x2 x, x, y, z; mov.b64 {%0, %1}, x; }"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// Barrier of a group's two warps (64 threads) that share a quarter of the
+// rows, and whether any of them sets `x`; of all softmax warps.
+__device__ __forceinline__ void pair_sync(int q) { asm volatile("barrier.cta.sync %0, 64;" ::"r"(q + 1) : "memory"); }
+__device__ __forceinline__ void soft_sync() { asm volatile("barrier.cta.sync 9, %0;" ::"n"(kSoftWarps * 32) : "memory"); }
+__device__ __forceinline__ bool pair_any(int q, bool x) {
+  uint32_t r;
+  asm volatile(
+      "{ .reg .pred p, c; setp.ne.u32 c, %2, 0; barrier.cta.red.or.pred p, %1, 64, c; selp.u32 %0, 1, 0, p; }"
+      : "=r"(r)
+      : "r"(q + 1), "r"((uint32_t)x)
+      : "memory");
+  return r != 0;
+}
 
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
@@ -142,9 +208,10 @@ template <int HD, int FMT, bool F32Q>
 __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
     kv_attend_wide_kernel(const __grid_constant__ KvAttnArgs a, const bool vec) {
   using G_ = Geo<HD, FMT, F32Q>;
-  constexpr int R = G_::kRing, TB = G_::kTileBytes;
-  __shared__ __align__(8) uint64_t kfull[R], kempty[R], vfull[R], vempty[R], sfull[2], pfull[2], odone, qfull, drained;
+  constexpr int R = G_::kRing, TB = G_::kTileBytes, NS = G_::kStages, SB = G_::kStage;
+  __shared__ __align__(8) uint64_t kfull[R], kempty[R], vfull[R], vempty[R], sfull[2], pfull[2], odone, qfull, decided, drained;
   __shared__ __align__(8) uint64_t scfull[kScaleRing], scempty[kScaleRing];
+  __shared__ __align__(8) uint64_t stfull[2 * NS], stempty[2 * NS];  // stages of keys, then of values
   __shared__ uint32_t tmem_s;
   __shared__ int abort_s;
   extern __shared__ uint8_t smem_raw[];
@@ -152,7 +219,12 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
   uint8_t* kring = smem;
   uint8_t* vring = smem + R * TB;
   uint8_t* qlo = vring + R * TB;
-  float* scales = reinterpret_cast<float*>(qlo + G_::kQlo);  // [ring][keys 64, values 64, exponent, pad]
+  uint8_t* stages = qlo + G_::kQlo;                                 // [keys, values][stage]
+  float* scales = reinterpret_cast<float*>(stages + 2 * NS * SB);  // [ring][keys 64, values 64, exponent, pad]
+  float* tops = scales + kScaleRing * (2 * kT + 4);  // [half][row] maxima of a tile
+  float* mrow = tops + 2 * kM;                       // [row] maximum
+  int* erow = reinterpret_cast<int*>(mrow + kM);     // [row] exponent
+  float* sums = reinterpret_cast<float*>(erow + kM); // [2][row]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const KvPool& p = a.pool;
@@ -175,14 +247,19 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
     }
     for (int b = 0; b < 2; b++) {
       bar_init(&sfull[b], 1);
-      bar_init(&pfull[b], 4);
+      bar_init(&pfull[b], 8);
     }
     for (int s = 0; s < kScaleRing; s++) {
-      bar_init(&scfull[s], FMT == kKvI8 ? 2 : 1);
-      bar_init(&scempty[s], 4);
+      bar_init(&scfull[s], 2);
+      bar_init(&scempty[s], 8);
+    }
+    for (int s = 0; s < 2 * NS; s++) {
+      bar_init(&stfull[s], 1);
+      bar_init(&stempty[s], 4);
     }
     bar_init(&odone, 1);
-    bar_init(&qfull, 4);
+    bar_init(&qfull, kSoftWarps);
+    bar_init(&decided, 8);
     bar_init(&drained, 1);
     abort_s = 0;
     bar_init_fence();
@@ -204,22 +281,23 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
   };
   // a warp's wait: one outcome for all lanes
   auto wait = [&](uint64_t* b, uint32_t parity) {
-    if (__any_sync(0xffffffffu, *abort_v)) return false;
-    const bool ok = __all_sync(0xffffffffu, bar_wait(b, parity, kWaitLimit));
-    if (!ok) give_up();
-    return ok;
+    for (int i = 0; i < kWaitLimit; i++) {
+      if (__all_sync(0xffffffffu, bar_try(b, parity))) return true;
+      if ((i & 31) == 31 && __any_sync(0xffffffffu, *abort_v)) return false;
+    }
+    give_up();
+    return false;
   };
 
-  if (warp < 4) {
+  if (warp < kSoftWarps) {
     // ------------------------------------------------------- query rows
     // Row by row with the lanes along the head; first parts go through the V
     // ring (chunks XOR-ed with the row) to the thread that owns the row.
-    const int r0 = warp * 32;
-    float cq = 0.f;
-    int rp = -1;
+    const int quarter = warp & 3, half = (warp >> 2) & 1, grp = warp >> 3, r0 = quarter * 32;
+    const int pair = grp * 4 + quarter, part = warp >> 2;
     {
-      constexpr int N = HD / 32, U = 8;  // U rows in flight
-      for (int rb = 0; rb < 32; rb += U) {
+      constexpr int N = HD / 32, U = 4;  // rows in flight
+      for (int rb = 8 * part; rb < 8 * part + 8; rb += U) {
         float x[U][N];
 #pragma unroll
         for (int u = 0; u < U; u++) {
@@ -238,7 +316,7 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
-          const int row = r0 + rb + u, rr = tr.r0 + row;
+          const int row = r0 + rb + u;
           uint32_t m = 0;
 #pragma unroll
           for (int j = 0; j < N; j++) m = max(m, __float_as_uint(x[u][j]) & 0x7fffffffu);
@@ -264,25 +342,32 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
             *reinterpret_cast<uint32_t*>(d) = *reinterpret_cast<const uint32_t*>(hi);
             if constexpr (F32Q) *reinterpret_cast<uint32_t*>(dl) = *reinterpret_cast<const uint32_t*>(lo);
           }
-          if (lane == rb + u) {
-            cq = fmaxf(pow2i(e) * fabsf(a.scale_log2e), FLT_MIN);  // never 0: hidden scores stay -inf
-            if (rr < tr.nr) rp = (int)max(min(tr.pos + rr / group, (int64_t)INT_MAX), (int64_t)-1);
-          }
+          if (lane == 0) tops[row] = fmaxf(pow2i(e) * fabsf(a.scale_log2e), FLT_MIN);  // never 0: hidden scores stay -inf
         }
       }
     }
-    __syncwarp();
-    const int row = r0 + lane;
+    soft_sync();
+    const int row = r0 + lane, rr = tr.r0 + row;
+    const bool live = rr < tr.nr;
     const uint32_t lanes = tmem + ((uint32_t)r0 << 16);
+    const float cq = tops[row];
+    int rp = -1;
+    if (live) rp = (int)max(min(tr.pos + rr / group, (int64_t)INT_MAX), (int64_t)-1);
+    // the four warps of a quarter move a fourth of its Q each
+    constexpr int kQC = HD / 32;  // 16-byte chunks
 #pragma unroll
-    for (int b = 0; b < HD / 64; b++) {
-      uint32_t v[32];
+    for (int c = 0; c < kQC; c += 2) {
+      uint32_t v[8];
 #pragma unroll
-      for (int c = 0; c < 8; c++) {
-        const uint4 w = *reinterpret_cast<const uint4*>(vring + row * HD * 2 + (((b * 8 + c) ^ (row & 7)) << 4));
-        v[4 * c] = w.x, v[4 * c + 1] = w.y, v[4 * c + 2] = w.z, v[4 * c + 3] = w.w;
+      for (int k = 0; k < 2; k++) {
+        const uint4 w = *reinterpret_cast<const uint4*>(vring + row * HD * 2 + (((part * kQC + c + k) ^ (row & 7)) << 4));
+        v[4 * k] = w.x, v[4 * k + 1] = w.y, v[4 * k + 2] = w.z, v[4 * k + 3] = w.w;
       }
-      tmem_st32(lanes + G_::kTmemQ + 32 * b, v);
+      tmem_st8(lanes + G_::kTmemQ + 4 * (part * kQC + c), v);
+    }
+    if (part == 0) {
+      mrow[row] = -INFINITY;
+      erow[row] = -100;
     }
     tmem_wait_st();
     tc_before();
@@ -291,99 +376,132 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
     if (lane == 0) bar_arrive(&qfull);
 
     // ----------------------------------------------------------- softmax
-    float m = -INFINITY, l = 0.f;
+    soft_sync();  // mrow and erow are set
+    float m = -INFINITY;
+    float2 l2 = make_float2(0.f, 0.f);
     int ev = -100;
     bool ok = true;
-    int it = 0;
+    int it = 0, mine = -1;  // tiles so far, the group's last
     for (int ti = sp.first; ti < sp.end; ti = sp.next(ti), it++) {
-      const int b = it & 1, sr = it % kScaleRing, t0 = ti * kT;
+      if ((it & 1) != grp) continue;
+      mine = it;
+      const int b = it & 1, sr = it % kScaleRing, t0 = ti * kT + 32 * half;
       const float* sc = scales + sr * (2 * kT + 4);
-      ok = wait(&scfull[sr], (it / kScaleRing) & 1) && wait(&sfull[b], (it >> 1) & 1);
-      if (!ok) break;
+      // A wait that ran out is told to the pair's other warp at its barrier,
+      // so that no warp is left in one.
+      ok = ok && wait(&scfull[sr], (it / kScaleRing) & 1) && wait(&sfull[b], (it >> 1) & 1);
       tc_after();
       const uint32_t st = lanes + G_::kTmemS + b * kT;
-      uint32_t s0[32], s1[32];
-      tmem_ld32(st, s0);
-      tmem_ld32(st + 32, s1);
+      uint32_t s0[32];
+      tmem_ld32(st + 32 * half, s0);
+      float2 x[16];
+      const float4* ks = reinterpret_cast<const float4*>(sc + 32 * half);
+      const int et = __float_as_int(sc[2 * kT]);
       tmem_wait(s0);
-      tmem_wait(s1);
-      float x[kT];
 #pragma unroll
-      for (int j = 0; j < 32; j += 4) {
-        const float4 k0 = *reinterpret_cast<const float4*>(sc + j), k1 = *reinterpret_cast<const float4*>(sc + 32 + j);
-        x[j] = __uint_as_float(s0[j]) * k0.x, x[j + 1] = __uint_as_float(s0[j + 1]) * k0.y;
-        x[j + 2] = __uint_as_float(s0[j + 2]) * k0.z, x[j + 3] = __uint_as_float(s0[j + 3]) * k0.w;
-        x[32 + j] = __uint_as_float(s1[j]) * k1.x, x[33 + j] = __uint_as_float(s1[j + 1]) * k1.y;
-        x[34 + j] = __uint_as_float(s1[j + 2]) * k1.z, x[35 + j] = __uint_as_float(s1[j + 3]) * k1.w;
+      for (int j = 0; j < 8; j++) {
+        const float4 k = ks[j];
+        x[2 * j] = mul2(make_float2(__uint_as_float(s0[4 * j]), __uint_as_float(s0[4 * j + 1])), make_float2(k.x, k.y));
+        x[2 * j + 1] = mul2(make_float2(__uint_as_float(s0[4 * j + 2]), __uint_as_float(s0[4 * j + 3])), make_float2(k.z, k.w));
       }
-      const bool whole = sp.whole(t0, kT);
-      uint64_t hidden = 0;
+      const bool whole = sp.whole(ti * kT, kT);
       if (!whole) {
 #pragma unroll
-        for (int j = 0; j < kT; j++)
-          if (!sp.sees(rp, t0 + j)) {
-            x[j] = -INFINITY;
-            hidden |= 1ull << j;
-          }
+        for (int j = 0; j < 16; j++) {
+          if (!sp.sees(rp, t0 + 2 * j)) x[j].x = -INFINITY;
+          if (!sp.sees(rp, t0 + 2 * j + 1)) x[j].y = -INFINITY;
+        }
       }
-      float mt[8];
+      float m4[4];
 #pragma unroll
-      for (int j = 0; j < 8; j++) mt[j] = x[j];
+      for (int j = 0; j < 4; j++) m4[j] = fmaxf(x[j].x, x[j].y);
 #pragma unroll
-      for (int j = 8; j < kT; j++) mt[j & 7] = fmaxf(mt[j & 7], x[j]);
-      const float mx = fmaxf(fmaxf(fmaxf(mt[0], mt[1]), fmaxf(mt[2], mt[3])), fmaxf(fmaxf(mt[4], mt[5]), fmaxf(mt[6], mt[7]))) * cq;
-      // the maximum and the exponent move only when weights could overflow
-      const float mn = mx > m + 8.f || m == -INFINITY ? mx : m;
-      const float ms = mn == -INFINITY ? 0.f : mn;
-      const int et = __float_as_int(sc[2 * kT]);
+      for (int j = 4; j < 16; j++) m4[j & 3] = max3(m4[j & 3], x[j].x, x[j].y);
+      float mx = fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]) * cq;
+      if (it > 0) {  // the other group's decision on the tile before
+        ok = ok && wait(&decided, (it - 1) & 1);
+        const float mo = mrow[row];
+        const int eo = erow[row];
+        if (mo != m || eo != ev) {
+          const float f = m == -INFINITY ? 0.f : ex2(m - mo + (float)(ev - eo));
+          l2 = mul2(l2, make_float2(f, f));
+          m = mo;
+          ev = eo;
+        }
+      }
+      // both threads of a row have read its scores when the barrier opens
+      const bool move = mx > m + 8.f || m == -INFINITY;
       const int en = et > ev ? et + 2 : ev;
-      const float alpha = m == mn ? 1.f : ex2(m - ms);
-      const float fo = alpha * (ev - en < -126 ? 0.f : pow2i(max(ev - en, -126)));
-      m = mn;
-      ev = en;
-      l *= alpha;
-      const float up = pow2i(-en) * 128.f;
-      uint32_t w[32];
-      uint32_t wl[F32Q ? 32 : 1];
-      float la[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int j = 0; j < kT; j += 4) {
-        const float4 vs = *reinterpret_cast<const float4*>(sc + kT + j);
-        const float p0 = ex2(fmaf(x[j], cq, -ms)), p1 = ex2(fmaf(x[j + 1], cq, -ms)), p2 = ex2(fmaf(x[j + 2], cq, -ms)),
-                    p3 = ex2(fmaf(x[j + 3], cq, -ms));
-        la[0] += p0, la[1] += p1, la[2] += p2, la[3] += p3;
-        float w0 = p0 * (vs.x * up), w1 = p1 * (vs.y * up), w2 = p2 * (vs.z * up), w3 = p3 * (vs.w * up);
-        if (!whole) {  // a hidden token weighs zero whatever its scale is
-          if (hidden >> j & 1) w0 = 0.f;
-          if (hidden >> (j + 1) & 1) w1 = 0.f;
-          if (hidden >> (j + 2) & 1) w2 = 0.f;
-          if (hidden >> (j + 3) & 1) w3 = 0.f;
+      float fo = 1.f;
+      if (pair_any(pair, move || !ok) || en != ev) {
+        tops[half * kM + row] = mx;
+        sums[half * kM + row] = ok ? 0.f : 1.f;
+        pair_sync(pair);
+        mx = fmaxf(mx, tops[(half ^ 1) * kM + row]);
+        const bool other = sums[(half ^ 1) * kM + row] == 0.f;
+        pair_sync(pair);
+        if (!__all_sync(0xffffffffu, ok && other)) {
+          ok = false;
+          break;
         }
-        w[j / 2] = pack2(w0, w1);
-        w[j / 2 + 1] = pack2(w2, w3);
-        if constexpr (F32Q) {
-          const float2 f0 = unpack2(w[j / 2]), f1 = unpack2(w[j / 2 + 1]);
-          wl[j / 2] = pack2(w0 - f0.x, w1 - f0.y);
-          wl[j / 2 + 1] = pack2(w2 - f1.x, w3 - f1.y);
+        const float mn = mx > m + 8.f || m == -INFINITY ? mx : m;
+        // o and l by 2^(old reference - new)
+        const float d = (m == -INFINITY ? 0.f : m) - (mn == -INFINITY ? 0.f : mn) + (float)(ev - en);
+        fo = m == mn && en == ev ? 1.f : m == -INFINITY ? 0.f : ex2(d);
+        m = mn;
+        ev = en;
+        l2 = mul2(l2, make_float2(fo, fo));
+        if (half == 0) {
+          mrow[row] = m;
+          erow[row] = ev;
         }
       }
-      l += (la[0] + la[1]) + (la[2] + la[3]);
+      __syncwarp();
+      if (lane == 0) bar_arrive(&decided);
+      const float r = (m == -INFINITY ? 0.f : m) - 7.f + (float)ev;
+      const float4* vs = reinterpret_cast<const float4*>(sc + kT + 32 * half);
+#pragma unroll
+      for (int hh = 0; hh < 2; hh++) {
+        uint32_t w[8], wl[8];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const float4 v = vs[4 * hh + j];
+          const float2 x0 = x[8 * hh + 2 * j], x1 = x[8 * hh + 2 * j + 1];
+          float2 a0 = fma2(x0, make_float2(cq, cq), make_float2(-r, -r)),
+                 a1 = fma2(x1, make_float2(cq, cq), make_float2(-r, -r));
+          a0 = make_float2(ex2(a0.x), ex2(a0.y));
+          a1 = make_float2(ex2(a1.x), ex2(a1.y));
+          l2 = add2(l2, add2(a0, a1));
+          float2 w0 = mul2(a0, make_float2(v.x, v.y)), w1 = mul2(a1, make_float2(v.z, v.w));
+          if (!whole) {  // a hidden token weighs zero whatever its scale is
+            if (x0.x == -INFINITY) w0.x = 0.f;
+            if (x0.y == -INFINITY) w0.y = 0.f;
+            if (x1.x == -INFINITY) w1.x = 0.f;
+            if (x1.y == -INFINITY) w1.y = 0.f;
+          }
+          w[2 * j] = pack2(w0.x, w0.y);
+          w[2 * j + 1] = pack2(w1.x, w1.y);
+          if constexpr (F32Q) {
+            const float2 f0 = unpack2(w[2 * j]), f1 = unpack2(w[2 * j + 1]);
+            wl[2 * j] = pack2(w0.x - f0.x, w0.y - f0.y);
+            wl[2 * j + 1] = pack2(w1.x - f1.x, w1.y - f1.y);
+          }
+        }
+        tmem_st8(st + 16 * half + 8 * hh, w);
+        if constexpr (F32Q) tmem_st8(st + 32 + 16 * half + 8 * hh, wl);
+      }
       __syncwarp();
       if (lane == 0) bar_arrive(&scempty[sr]);
-      tmem_st32(st, w);
-      if constexpr (F32Q) tmem_st32(st + 32, wl);
       if (it > 0 && __any_sync(0xffffffffu, fo != 1.f)) {
         ok = wait(&odone, (it - 1) & 1);  // the previous product has been added
-        if (!ok) break;
         tc_after();
 #pragma unroll 1
-        for (int c = 0; c < HD; c += 32) {
-          uint32_t o[32];
-          tmem_ld32(lanes + c, o);
-          tmem_wait(o);
+        for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 16) {
+          uint32_t o[16];
+          tmem_ld16(lanes + c, o);
 #pragma unroll
-          for (int j = 0; j < 32; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * fo);
-          tmem_st32(lanes + c, o);
+          for (int j = 0; j < 16; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * fo);
+          tmem_st16(lanes + c, o);
         }
       }
       tmem_wait_st();
@@ -393,38 +511,47 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
     }
     // ----------------------------------------------------------- results
     tmem_wait_st();  // no store in flight past this point
-    // The last tile's scores say that the product two tiles back was added, so
-    // the two after it are waited for in turn: a parity names a phase only
-    // while no other of its kind is outstanding.
-    if (ok && it > 1) ok = wait(&odone, it & 1);
-    if (ok && it > 0) ok = wait(&odone, (it - 1) & 1);
+    // Every product has been added when `drained` fires (its only phase; odone
+    // may be two phases on by now, and a parity cannot tell).
+    ok = ok && wait(&drained, 0);
+    if (ok && it > 0 && mine != it - 1) {  // the last decision was the other group's
+      const float mo = mrow[row];
+      const int eo = erow[row];
+      const float f = mo == m && eo == ev ? 1.f : m == -INFINITY ? 0.f : ex2(m - mo + (float)(ev - eo));
+      l2 = mul2(l2, make_float2(f, f));
+      m = mo;
+      ev = eo;
+    }
+    // (a group that gave up leaves the others to their own waits: every
+    // thread of the softmax warps comes here)
+    soft_sync();
+    float* ls = half ? sums : tops;  // [group][row]
+    ls[grp * kM + row] = l2.x + l2.y;
+    soft_sync();
     if (ok && !__any_sync(0xffffffffu, *abort_v)) {
       tc_after();
-      const int rr = tr.r0 + row;
+      const float l = (tops[row] + tops[kM + row]) + (sums[row] + sums[kM + row]);
       const int grow = tr.row0 + rr / group, h = kvh * group + rr % group;
       const int64_t rh = (int64_t)grow * a.heads + h;
-      const bool live = rr < tr.nr;
-      const float f = a.slots > 1 ? 0x1p-7f : l != 0.f ? __fdiv_rn(0x1p-7f, l) : 0.f;
-      const float back = pow2i(ev);
-      if (a.slots > 1 && live) a.ml[rh * a.slots + slot] = make_float2(m, l);
+      const float f = a.slots > 1 ? 1.f : l != 0.f ? __fdiv_rn(1.f, l) : 0.f;
+      if (a.slots > 1 && live && part == 0) a.ml[rh * a.slots + slot] = make_float2(m - 7.f + (float)ev, l);
       auto put = [&](auto* dst, bool v16) {
         using T = std::remove_reference_t<decltype(*dst)>;
 #pragma unroll 1
-        for (int c = 0; c < HD; c += 32) {
-          uint32_t o[32];
+        for (int c = part * (HD / 4); c < (part + 1) * (HD / 4); c += 16) {
+          uint32_t o[16];
           if (it > 0) {
-            tmem_ld32(lanes + c, o);
-            tmem_wait(o);
+            tmem_ld16(lanes + c, o);
           } else {
 #pragma unroll
-            for (int j = 0; j < 32; j++) o[j] = 0;
+            for (int j = 0; j < 16; j++) o[j] = 0;
           }
           if (!live) continue;
 #pragma unroll
-          for (int j = 0; j < 32; j += 8) {
+          for (int j = 0; j < 16; j += 8) {
             float y[8];
 #pragma unroll
-            for (int k = 0; k < 8; k++) y[k] = __uint_as_float(o[j + k]) * back * f;
+            for (int k = 0; k < 8; k++) y[k] = __uint_as_float(o[j + k]) * f;
             store_n<T, 8>(dst + c + j, v16, y);
           }
         }
@@ -440,13 +567,15 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
     // The whole warp waits, one lane issues.
     constexpr uint32_t dS = idesc(kT, false), dO = idesc(HD, true);
     const uint32_t k0 = su32(kring), v0 = su32(vring), ql = su32(qlo);
+    uint32_t leader;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(leader));
     bool ok = wait(&qfull, 0);
     tc_after();
     auto score = [&](int i) {
       const int s = i % R;
       if (!wait(&kfull[s], (i / R) & 1)) return false;
       tc_after();
-      if (lane == 0) {
+      if (leader) {
         const uint32_t d = tmem + G_::kTmemS + (i & 1) * kT, kb = k0 + s * TB;
 #pragma unroll
         for (int st = 0; st < HD / 16; st++)
@@ -472,7 +601,7 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
       ok = wait(&pfull[it & 1], (it >> 1) & 1) && wait(&vfull[s], (it / R) & 1);
       if (!ok) break;
       tc_after();
-      if (lane == 0) {
+      if (leader) {
         const uint32_t pa = tmem + G_::kTmemS + (it & 1) * kT, vb = v0 + s * TB;
 #pragma unroll
         for (int part = 0; part < (F32Q ? 2 : 1); part++)
@@ -484,178 +613,171 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
       }
       __syncwarp();
     }
-    if (lane == 0) commit(&drained);  // every product issued above has completed when this fires
+    if (leader) commit(&drained);  // every product issued above has completed when this fires
     __syncwarp();
     bar_wait(&drained, 0, kDrainLimit);
-  } else if constexpr (FMT == kKvF16) {
-    // ------------------------------------------------ bulk copies (f16)
-    const int rt = min(p.page_tokens, kT), runs = kT / rt;
-    const int64_t hb = kv_head_bytes(FMT, HD, p.page_tokens);
-    constexpr int kParts = HD / 64;
-    auto page_of = [&](int ti) {
-      const int64_t pos = (int64_t)ti * kT + (int64_t)lane * rt;
-      const bool in = lane < runs && pos < sp.tokens;
-      int page = in ? kv_page(p, a.b, tr.seq, pos) : -1;
-      const int first = __shfl_sync(0xffffffffu, page, 0);
-      if (!in) page = first;
-      return max(page, 0);
-    };
-    auto copy = [&](int ti, int page, const uint8_t* pool, uint8_t* dst, uint64_t* full) {
-      const int tp = (ti * kT) & (p.page_tokens - 1);
-      if (lane == 0) bar_expect(full, TB);
-      __syncwarp();
-      for (int c0 = 0; c0 < runs * kParts; c0 += 32) {
-        const int c = c0 + lane, run = min(c / kParts, runs - 1), part = c % kParts;
-        const int64_t at = (int64_t)__shfl_sync(0xffffffffu, page, run) * p.nkv + kvh;
-        if (c < runs * kParts)
-          bulk_load(su32(dst + (part * kT + run * rt) * 128), pool + at * hb + ((int64_t)part * p.page_tokens + tp) * 128,
-                    rt * 128, full);
-      }
-      __syncwarp();
-    };
-    // scales of two tokens a lane, and the exponent above the values'
-    auto put_scales = [&](int i, int ti, int page) {
-      const int sr = i % kScaleRing;
-      if (i >= kScaleRing && !wait(&scempty[sr], ((i / kScaleRing) + 1) & 1)) return false;
-      float* sc = scales + sr * (2 * kT + 4);
-      uint32_t top = 0;
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const int t = lane + 32 * h;
-        const int64_t at = ((int64_t)__shfl_sync(0xffffffffu, page, t / rt) * p.nkv + kvh) * p.page_tokens +
-                           ((ti * kT + t) & (p.page_tokens - 1));
-        const float v = p.vs[at];
-        sc[t] = p.ks[at];
-        sc[kT + t] = v;
-        const uint32_t bits = __float_as_uint(v);
-        if (bits < 0x7f800000u && ti * kT + t < sp.tokens) top = max(top, bits);
-      }
-      top = __reduce_max_sync(0xffffffffu, top);
-      if (lane == 0) sc[2 * kT] = __int_as_float(max((int)(top >> 23), 1) - 126);
-      __syncwarp();
-      if (lane == 0) bar_arrive(&scfull[sr]);
-      return true;
-    };
-    int it = 0, ti = sp.first, kn = 0, vn = 0;  // tiles of keys and values requested
-    bool ok = true;
-    if (ti < sp.end) {
-      int page = page_of(ti);
-      copy(ti, page, p.k, kring, &kfull[0]);
-      kn = 1;
-      ok = put_scales(0, ti, page);
-      for (; ok && ti < sp.end; it++) {
-        const int nt = sp.next(ti);
-        int npage = 0;
-        if (nt < sp.end) {
-          npage = page_of(nt);
-          const int s = (it + 1) % R;
-          if (it + 1 >= R && !(ok = wait(&kempty[s], (((it + 1) / R) + 1) & 1))) break;
-          copy(nt, npage, p.k, kring + s * TB, &kfull[s]);
-          kn = it + 2;
-          if (!(ok = put_scales(it + 1, nt, npage))) break;
-        }
-        const int s = it % R;
-        // the V ring holds the query rows first
-        if (it == 0 && !(ok = wait(&qfull, 0))) break;
-        if (it >= R && !(ok = wait(&vempty[s], ((it / R) + 1) & 1))) break;
-        copy(ti, page, p.v, vring + s * TB, &vfull[s]);
-        vn = it + 1;
-        ti = nt;
-        page = npage;
-      }
-    }
-    for (int s = 0; s < R; s++) {  // no copy outlives the CTA
-      if (kn > s) bar_wait(&kfull[(kn - 1 - s) % R], ((kn - 1 - s) / R) & 1, kDrainLimit);
-      if (vn > s) bar_wait(&vfull[(vn - 1 - s) % R], ((vn - 1 - s) / R) & 1, kDrainLimit);
-    }
-  } else {
-    // ------------------------------------------- expansion to f16 (i8)
-    // Warps 5-8 keys, 9-12 values; a thread takes HD / 32 16-byte chunks of a
-    // tile, all loaded before the ring's slot is waited for.
-    const int isv = (warp - kLoadWarp) >> 2, tid = threadIdx.x - (kLoadWarp + 4 * isv) * 32;
-    const bool first_warp = tid < 32;
+  } else if (warp < kExpandWarp) {
+    // ----------------------------------------------------- bulk copies
+    // A warp takes every other tile of keys or values.  The page ids of its
+    // next tile are read a turn ahead, that tile's scales likewise, and neither
+    // is looked at before then, so that no load is waited for.
+    const bool isv = (warp - kLoadWarp) & 1;
+    const int turn = (warp - kLoadWarp) >> 1;
     uint8_t* ring = isv ? vring : kring;
     uint64_t* full = isv ? vfull : kfull;
     uint64_t* empty = isv ? vempty : kempty;
     const uint8_t* pool = isv ? p.v : p.k;
     const float* spool = isv ? p.vs : p.ks;
+    const int rs = min(p.page_shift, 6), rt = 1 << rs, runs = kT >> rs;  // tokens of a page's run in a tile
     const int64_t hb = kv_head_bytes(FMT, HD, p.page_tokens);
-    const int rt = min(p.page_tokens, kT), runs = kT / rt;
-    constexpr int C = HD / 16, TP = 128 / C, NP = kT / TP;  // chunks a token, tokens a pass, passes
-    const int ch = tid % C, tk = tid / C;
-    auto page_of = [&](int ti) {
-      const int64_t pos = (int64_t)ti * kT + (int64_t)lane * rt;
-      const bool in = ti < sp.end && lane < runs && pos < sp.tokens;
-      int page = in ? kv_page(p, a.b, tr.seq, pos) : -1;
-      const int f = __shfl_sync(0xffffffffu, page, 0);
-      if (!in) page = f;
-      return max(page, 0);
+    auto holds = [&](int ti) {  // whether the lane's run of tile ti begins with a token of the sequence
+      return ti < sp.end && lane < runs && ti * kT + lane * rt < sp.tokens;
     };
-    uint4 raw[NP];
+    auto ask = [&](int ti) {
+      const int col = (ti * kT + lane * rt) >> p.page_shift;  // inside the table: below sp.tokens
+      return holds(ti) ? __ldg(a.b.table + (int64_t)tr.seq * a.b.table_ld + col) : -1;
+    };
+    auto page_of = [&](int ti, int id) {
+      if (holds(ti) && (id < 0 || id >= p.pages)) {
+        atomicOr(p.flag, kKvBadPage);
+        id = 0;
+      }
+      // runs behind the last token are filled from the tile's first page
+      const int first = __shfl_sync(0xffffffffu, id, 0);
+      return holds(ti) ? id : max(first, 0);
+    };
     float sv[2] = {0.f, 0.f};
-    auto load = [&](int ti, int page) {
+    auto load_scales = [&](int ti, int page) {
 #pragma unroll
-      for (int i = 0; i < NP; i++) {
-        const int t = i * TP + tk;  // physical chunk ch of token t
-        const int64_t at = (int64_t)__shfl_sync(0xffffffffu, page, t / rt) * p.nkv + kvh;
-        raw[i] = __ldg(reinterpret_cast<const uint4*>(pool + at * hb + (int64_t)((ti * kT + t) & (p.page_tokens - 1)) * HD + 16 * ch));
-      }
-      if (first_warp) {
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-          const int t = lane + 32 * h;
-          const int64_t at = (int64_t)__shfl_sync(0xffffffffu, page, t / rt) * p.nkv + kvh;
-          sv[h] = spool[at * p.page_tokens + ((ti * kT + t) & (p.page_tokens - 1))];
-        }
+      for (int h = 0; h < 2; h++) {
+        const int t = lane + 32 * h;
+        const int64_t at = (int64_t)__shfl_sync(0xffffffffu, page, t >> rs) * p.nkv + kvh;
+        sv[h] = spool[at * p.page_tokens + ((ti * kT + t) & (p.page_tokens - 1))];
       }
     };
+    // (Turns need a warp to know, from the fill it waited for last, that a
+    // barrier is at most one phase behind the one it waits for.  Two tiles
+    // apart that holds for rings of whole tiles, which are emptied in order; in
+    // a ring of three quarter tiles it does not: one warp fills those.)
+    constexpr bool kTurns = !(FMT == kKvI8 && G_::kSmall);
+    auto after = [&](int ti) { return kTurns ? sp.next(sp.next(ti)) : sp.next(ti); };
+    int it = turn, ti = !turn ? sp.first : kTurns ? sp.next(sp.first) : sp.end, t1 = after(ti);
+    bool ok = true;
+    int page = page_of(ti, ask(ti)), id1 = ask(t1);
+    if (ti < sp.end) load_scales(ti, page);
+    if (FMT == kKvF16 && isv && ti < sp.end) ok = wait(&qfull, 0);  // the V ring holds the query rows first
+    int requested = 0;  // one past the last fill of the ring (f16) or of the stages (i8)
+    for (; ok && ti < sp.end; it += kTurns ? 2 : 1) {
+      // the tile's scales and the exponent above the values'
+      const int sr = it % kScaleRing;
+      if (it >= kScaleRing && !(ok = wait(&scempty[sr], ((it / kScaleRing) + 1) & 1))) break;
+      float* sc = scales + sr * (2 * kT + 4);
+      uint32_t top = 0;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int t = lane + 32 * h;
+        sc[isv * kT + t] = sv[h];
+        const uint32_t bits = __float_as_uint(sv[h]);
+        if (bits < 0x7f800000u && ti * kT + t < sp.tokens) top = max(top, bits);
+      }
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (isv && lane == 0) sc[2 * kT] = __int_as_float(max((int)(top >> 23), 1) - 126);
+      __syncwarp();
+      if (lane == 0) bar_arrive(&scfull[sr]);
+      const int page1 = page_of(t1, id1), t2 = after(t1);
+      if (t1 < sp.end) load_scales(t1, page1);
+      id1 = ask(t2);
+      const int tp = (ti * kT) & (p.page_tokens - 1);
+      if constexpr (FMT == kKvF16) {
+        constexpr int kParts = HD / 64;
+        const int s = it % R;
+        if (it >= R && !(ok = wait(&empty[s], ((it / R) + 1) & 1))) break;
+        if (lane == 0) bar_expect(&full[s], TB);
+        __syncwarp();
+        requested = it + 1;
+#pragma unroll 1
+        for (int c0 = 0; c0 < runs * kParts; c0 += 32) {
+          const int c = c0 + lane, run = min(c / kParts, runs - 1), part = c % kParts;
+          const int64_t at = (int64_t)__shfl_sync(0xffffffffu, page, run) * p.nkv + kvh;
+          if (c < runs * kParts)
+            bulk_load(su32(ring + s * TB + (part * kT + run * rt) * 128),
+                      pool + at * hb + ((int64_t)part * p.page_tokens + tp) * 128, rt * 128, &full[s]);
+        }
+        __syncwarp();
+      } else {
+        constexpr int kPer = kT / G_::kStageTokens;  // stages of a tile
+        const int cs = min(rs, G_::kSmall ? 4 : 6), ct = 1 << cs, copies = G_::kStageTokens >> cs;
+#pragma unroll 1
+        for (int q = 0; q < kPer; q++) {
+          const int n = it * kPer + q, s = n % NS;
+          if (n >= NS && !(ok = wait(&stempty[isv * NS + s], ((n / NS) + 1) & 1))) break;
+          uint64_t* bar = &stfull[isv * NS + s];
+          if (lane == 0) bar_expect(bar, SB);
+          __syncwarp();
+          requested = n + 1;
+          const int t = q * G_::kStageTokens + min(lane, copies - 1) * ct;
+          const int64_t at = (int64_t)__shfl_sync(0xffffffffu, page, t >> rs) * p.nkv + kvh;
+          if (lane < copies)
+            bulk_load(su32(stages + (isv * NS + s) * SB + lane * ct * HD),
+                      pool + at * hb + (int64_t)((ti * kT + t) & (p.page_tokens - 1)) * HD, ct * HD, bar);
+          __syncwarp();
+        }
+        if (!ok) break;
+      }
+      ti = t1;
+      t1 = t2;
+      page = page1;
+    }
+    // Where every tile is used, its copy has landed.  Otherwise no copy may
+    // outlive the CTA: the last fills are waited for (again bounded).
+    if (!ok || __any_sync(0xffffffffu, *abort_v)) {
+      uint64_t* bars = FMT == kKvF16 ? full : stfull + isv * NS;
+      constexpr int kRound = FMT == kKvF16 ? R : NS;
+      for (int n = max(requested - 2 * kRound, 0); n < requested; n++) bar_wait(&bars[n % kRound], (n / kRound) & 1, 1 << 10);
+    }
+  } else {
+    // ------------------------------------------- expansion to f16 (i8)
+    // Four warps for keys, four for values; a thread takes 16-byte chunks.
+    const int isv = (warp - kExpandWarp) >> 2, tid = threadIdx.x - (kExpandWarp + 4 * isv) * 32;
+    uint8_t* ring = isv ? vring : kring;
+    uint64_t* full = isv ? vfull : kfull;
+    uint64_t* empty = isv ? vempty : kempty;
+    constexpr int C = HD / 16, TP = 128 / C;         // chunks a token, tokens a pass
+    constexpr int kPer = kT / G_::kStageTokens, NP = G_::kStageTokens / TP;  // stages a tile, passes a stage
+    const int ch = tid % C, tk = tid / C;
     bool ok = true;
     if (isv && sp.first < sp.end) ok = wait(&qfull, 0);  // the V ring holds the query rows first
-    int ti = sp.first, nt = sp.next(ti);
-    int page = ok && ti < sp.end ? page_of(ti) : 0;
-    if (ok && ti < sp.end) load(ti, page);
-    page = page_of(nt);
-    for (int it = 0; ok && ti < sp.end; it++) {
-      const int s = it % R, sr = it % kScaleRing;
-      const int nn = sp.next(nt), npage = page_of(nn);
-      if (first_warp) {
-        if (it >= kScaleRing && !(ok = wait(&scempty[sr], ((it / kScaleRing) + 1) & 1))) break;
-        float* sc = scales + sr * (2 * kT + 4);
-        uint32_t top = 0;
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-          const int t = lane + 32 * h;
-          sc[isv * kT + t] = sv[h];
-          const uint32_t bits = __float_as_uint(sv[h]);
-          if (bits < 0x7f800000u && ti * kT + t < sp.tokens) top = max(top, bits);
-        }
-        top = __reduce_max_sync(0xffffffffu, top);
-        if (isv && lane == 0) sc[2 * kT] = __int_as_float(max((int)(top >> 23), 1) - 126);
-        __syncwarp();
-        if (lane == 0) bar_arrive(&scfull[sr]);
-      }
+    int it = 0;
+    for (int ti = sp.first; ok && ti < sp.end; ti = sp.next(ti), it++) {
+      const int s = it % R;
       if (it >= R && !(ok = wait(&empty[s], ((it / R) + 1) & 1))) break;
       uint8_t* dst = ring + s * TB;
 #pragma unroll
-      for (int i = 0; i < NP; i++) {
-        const int t = i * TP + tk, c = ch ^ i8_swizzle(t, HD);  // its 16 elements are chunks 2c and 2c + 1 of the f16 row
-        const uint2 x0 = biased4_to_f16(raw[i].x), x1 = biased4_to_f16(raw[i].y), x2 = biased4_to_f16(raw[i].z),
-                    x3 = biased4_to_f16(raw[i].w);
-        const uint4 lo = make_uint4(x0.x, x0.y, x1.x, x1.y), hi = make_uint4(x2.x, x2.y, x3.x, x3.y);
-        uint8_t* rowp = dst + ((c >> 2) * kT + t) * 128;
-        // the two 64-element blocks that a quarter warp meets take their halves
-        // in turn, so that its eight stores fall on different banks
-        const int turn = (c >> 2) & 1, c8 = (c & 3) * 2;
-        *reinterpret_cast<uint4*>(rowp + (((c8 + turn) ^ (t & 7)) << 4)) = turn ? hi : lo;
-        *reinterpret_cast<uint4*>(rowp + (((c8 + 1 - turn) ^ (t & 7)) << 4)) = turn ? lo : hi;
+      for (int q = 0; q < kPer; q++) {
+        const int n = it * kPer + q, sn = n % NS;
+        if (!(ok = wait(&stfull[isv * NS + sn], (n / NS) & 1))) break;
+        const uint8_t* src = stages + (isv * NS + sn) * SB + tid * 16;
+#pragma unroll
+        for (int i = 0; i < NP; i++) {
+          const uint4 raw = *reinterpret_cast<const uint4*>(src + 2048 * i);
+          const int t = (NP * q + i) * TP + tk, c = ch ^ i8_swizzle(t, HD);  // 16 elements: chunks 2c, 2c + 1 of the f16 row
+          const uint2 y0 = biased4_to_f16(raw.x), y1 = biased4_to_f16(raw.y), y2 = biased4_to_f16(raw.z),
+                      y3 = biased4_to_f16(raw.w);
+          const uint4 lo = make_uint4(y0.x, y0.y, y1.x, y1.y), hi = make_uint4(y2.x, y2.y, y3.x, y3.y);
+          uint8_t* rowp = dst + ((c >> 2) * kT + t) * 128;
+          // the two 64-element blocks that a quarter warp meets take their
+          // halves in turn, so that its eight stores fall on different banks
+          const int turn = (c >> 2) & 1, c8 = (c & 3) * 2;
+          *reinterpret_cast<uint4*>(rowp + (((c8 + turn) ^ (t & 7)) << 4)) = turn ? hi : lo;
+          *reinterpret_cast<uint4*>(rowp + (((c8 + 1 - turn) ^ (t & 7)) << 4)) = turn ? lo : hi;
+        }
+        __syncwarp();
+        if (lane == 0) bar_arrive(&stempty[isv * NS + sn]);
       }
+      if (!ok) break;
       async_fence();
       __syncwarp();
       if (lane == 0) bar_arrive(&full[s]);
-      if (nt < sp.end) load(nt, page);
-      ti = nt;
-      nt = nn;
-      page = npage;
     }
   }
   __syncwarp();

@@ -19,17 +19,22 @@ __device__ __forceinline__ void bar_arrive(uint64_t* b) {
 __device__ __forceinline__ void bar_expect(uint64_t* b, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(su32(b)), "r"(bytes) : "memory");
 }
-// Bounded wait for the phase of `parity`; false when it ran out.
+// Whether the phase of `parity` completes within about 2 us: the thread sleeps
+// until then, so that waiting warps leave the issue slots to the others (with
+// no time given, 27 warps' polls were over half of a kernel's instructions).
+constexpr uint32_t kWaitNs = 2000;
+__device__ __forceinline__ bool bar_try(uint64_t* b, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }"
+               : "=r"(ok)
+               : "r"(su32(b)), "r"(parity), "r"(kWaitNs)
+               : "memory");
+  return ok;
+}
+// Bounded wait; false when it ran out.
 __device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, int limit) {
-  const uint32_t a = su32(b);
-  for (int i = 0; i < limit; i++) {
-    uint32_t ok;
-    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-                 : "=r"(ok)
-                 : "r"(a), "r"(parity)
-                 : "memory");
-    if (ok) return true;
-  }
+  for (int i = 0; i < limit; i++)
+    if (bar_try(b, parity)) return true;
   return false;
 }
 // 1-D bulk copy global -> shared of this GPU's memory; both addresses and the
