@@ -204,6 +204,16 @@ int iq_model_weight_bytes(const iq_model* m, int64_t* bytes);
 /* Decode state: per-layer KV cache (f32 [pos][kv_head][head_dim]) and
  * DeltaNet conv/recurrent state, double-buffered for rollback. */
 int iq_state_create(iq_model* m, int64_t max_positions, iq_state** out);
+/* The same with the KV cache of every attention layer (and the MTP block) in
+ * `kv_format`: IQ_F32 as above, or a paged cache of IQ_F16 or IQ_I8 vectors
+ * (see iq_kv_create: half or a quarter of the bytes).  With window > 0 (F16 or
+ * I8 only) a row attends to its last `window` positions and to the first
+ * `sinks` ones; the cache still holds all.  Passes of up to 8 rows keep their
+ * property that a row's result depends on its own context only; state images
+ * are the same f32 images, whichever format exports or imports them. */
+int iq_state_create_kv(iq_model* m, int64_t max_positions, int kv_format, int window, int sinks, iq_state** out);
+/* Device bytes of the state's KV caches. */
+int iq_state_kv_bytes(const iq_state* s, int64_t* bytes);
 void iq_state_destroy(iq_state* s);
 int iq_state_reset(iq_state* s);
 int iq_state_position(const iq_state* s, int64_t* position);

@@ -59,6 +59,7 @@ struct KvAttnArgs {
   int window, sinks;   // window 0: none
   int chunk;           // tokens per split, a multiple of 64
   int slots;           // splits that a tile of query rows can need
+  bool narrow;         // never the tensor-core kernel (its rows' results depend on the launch)
   float* part;         // slots > 1: [row][head][slot][hd] unnormalised outputs
   float2* ml;          //            [row][head][slot] {maximum, sum}, base-2 exponents
 };
@@ -82,6 +83,14 @@ size_t kv_attend_plan(KvAttnArgs& a, int max_rows);
 void kv_attend_bind(KvAttnArgs& a, void* workspace);
 cudaError_t kv_attend_launch(const KvAttnArgs& a, int max_rows, cudaStream_t st);
 
+}  // namespace iq
+
+struct iq_kv;
+namespace iq {
+// Allocates and clears a cache on the current device (iq_kv_create's part
+// behind its checks).  `flag`: where errors are recorded, NULL for a word of
+// its own.
+int kv_create(int format, int kv_heads, int head_dim, int page_tokens, int64_t pages, int* flag, iq_kv& c);
 }  // namespace iq
 
 struct iq_kv {

@@ -500,80 +500,136 @@ __global__ void __launch_bounds__(160) kv_attend_kernel(const __grid_constant__ 
 }
 
 // A row's splits joined: out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c
-// over the chunks c that the row sees.  One CTA per (row, head); chunk c goes
-// to thread group c mod NG, whose sums are joined in order, so the result
-// depends on the row's own chunks only.
+// over the chunks c that the row sees.  Chunk c belongs to group c mod 8; a
+// group's chunks are summed in order, then the groups in order, whichever
+// kernel does it: the result depends on the row's own chunks only.
+constexpr int kGroups = 8, kFewSlots = 32;
+
+struct JoinRow {
+  KvChunks ch;
+  KvRowChunks rc;
+  int64_t rh;
+};
+// False for a row behind the last sequence.  Warp-wide.
+__device__ __forceinline__ bool join_row(const KvAttnArgs& a, int row, int h, int tq, int lane, JoinRow* j) {
+  int i;
+  const int seq = kv_seq_of_row(a.b, row, lane, &i);
+  if (seq < 0) return false;
+  const int group = a.heads / a.pool.nkv;
+  const int64_t base = a.b.position[seq];
+  const int tile0 = (i * group + h % group) / tq * tq;  // the row's tile begins here
+  j->ch = kv_chunks(a, base + tile0 / group);
+  j->rc = kv_row_chunks(a, j->ch, base + i);
+  j->rh = (int64_t)row * a.heads + h;
+  return true;
+}
+// acc and sum of the group's chunks lo .. hi - 1 of the row (weights w(c)).
+template <int N, class W>
+__device__ __forceinline__ void join_group(const JoinRow& j, int slots, const float* part, const float2* ml, int hd,
+                                           int lane, int g, int lo, int hi, W weight, float (&acc)[N], float& sum) {
+  for (int r = 0; r < 2; r++) {  // the always-visible chunks, then the window's
+    const int b = max(lo, r ? j.rc.firsts : 0), e = min(hi, r ? j.rc.count : j.rc.firsts);
+    if (b >= e) continue;
+    const int first = j.rc.chunk(b);
+#pragma unroll 2
+    for (int c = b + ((g - first) & (kGroups - 1)); c < e; c += kGroups) {
+      const int64_t at = j.rh * slots + j.ch.slot(j.rc.chunk(c));
+      const float w = weight(c);
+      float x[N];
+      load_n<float, N>(part + at * hd + lane * N, true, x);
+#pragma unroll
+      for (int k = 0; k < N; k++) acc[k] = fmaf(w, x[k], acc[k]);
+      sum = fmaf(w, ml[at].y, sum);
+    }
+  }
+}
+
+// Up to 32 slots: one warp per (row, head).
+template <class T, int HD>
+__global__ void __launch_bounds__(256) kv_join_few_kernel(const __grid_constant__ KvAttnArgs a, const int tq,
+                                                          const bool vec) {
+  constexpr int N = HD / 32;
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int row = (int)(item / a.heads), h = (int)(item % a.heads);
+  if (row >= a.b.rows) return;
+  JoinRow j;
+  if (!join_row(a, row, h, tq, lane, &j)) return;
+  const float m = lane < j.rc.count ? a.ml[j.rh * a.slots + j.ch.slot(j.rc.chunk(lane))].x : -INFINITY;
+  float M = m;
+#pragma unroll
+  for (int w = 16; w; w >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, w));
+  const float wt = kvp::ex2(m - (M == -INFINITY ? 0.f : M));
+  float acc[N], sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < N; k++) acc[k] = 0.f;
+#pragma unroll 1
+  for (int g = 0; g < kGroups; g++) {
+    float x[N], s = 0.f;
+#pragma unroll
+    for (int k = 0; k < N; k++) x[k] = 0.f;
+    join_group<N>(j, a.slots, a.part, a.ml, HD, lane, g, 0, j.rc.count,
+                  [&](int c) { return __shfl_sync(0xffffffffu, wt, c); }, x, s);
+#pragma unroll
+    for (int k = 0; k < N; k++) acc[k] += x[k];
+    sum += s;
+  }
+  const float f = sum != 0.f ? __fdiv_rn(1.f, sum) : 0.f;
+#pragma unroll
+  for (int k = 0; k < N; k++) acc[k] *= f;
+  store_n<T, N>(static_cast<T*>(a.out.p) + (int64_t)row * a.out.row + (int64_t)h * a.out.head + lane * N, vec, acc);
+}
+
+// Any number of slots: one CTA per (row, head), a warp per group.
 template <class T, int HD>
 __global__ void __launch_bounds__(256) kv_join_kernel(const __grid_constant__ KvAttnArgs a, const int tq,
                                                       const bool vec) {
-  constexpr int TPG = HD / 4, NG = 256 / TPG, kWeights = 1024;
-  __shared__ float wt[kWeights], red[8], sums[NG];
-  __shared__ float4 os[NG][TPG];
+  constexpr int N = HD / 32, kWeights = 1024;
+  __shared__ float wt[kWeights], red[8], sums[kGroups], os[kGroups][HD];
   pdl_wait();
   const int row = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
-  const int lane = threadIdx.x & 31, grp = threadIdx.x / TPG, d4 = threadIdx.x % TPG;
-  int i;
-  const int seq = kv_seq_of_row(a.b, row, lane, &i);
-  if (seq < 0) return;
-  const int group = a.heads / a.pool.nkv;
-  const int64_t base = a.b.position[seq], pos = base + i;
-  const int tile0 = (i * group + h % group) / tq * tq;  // the row's tile begins here
-  const KvChunks ch = kv_chunks(a, base + tile0 / group);
-  const KvRowChunks rc = kv_row_chunks(a, ch, pos);
-  const int64_t rh = (int64_t)row * a.heads + h;
-  const float2* ml = a.ml + rh * a.slots;
-  const float* part = a.part + rh * a.slots * HD + 4 * d4;
+  const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
+  JoinRow j;
+  if (!join_row(a, row, h, tq, lane, &j)) return;
+  const float2* ml = a.ml + j.rh * a.slots;
   float mxv = -INFINITY;
-  for (int c = threadIdx.x; c < rc.count; c += 256) mxv = fmaxf(mxv, ml[ch.slot(rc.chunk(c))].x);
+  for (int c = threadIdx.x; c < j.rc.count; c += 256) mxv = fmaxf(mxv, ml[j.ch.slot(j.rc.chunk(c))].x);
 #pragma unroll
   for (int w = 16; w; w >>= 1) mxv = fmaxf(mxv, __shfl_xor_sync(0xffffffffu, mxv, w));
-  if (lane == 0) red[threadIdx.x >> 5] = mxv;
+  if (lane == 0) red[grp] = mxv;
   __syncthreads();
   float M = red[0];
 #pragma unroll
   for (int w = 1; w < 8; w++) M = fmaxf(M, red[w]);
   const float ms = M == -INFINITY ? 0.f : M;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float sum = 0.f;
-  for (int c0 = 0; c0 < rc.count; c0 += kWeights) {
-    const int nc = min(kWeights, rc.count - c0);
+  float acc[N], sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < N; k++) acc[k] = 0.f;
+  for (int c0 = 0; c0 < j.rc.count; c0 += kWeights) {
+    const int nc = min(kWeights, j.rc.count - c0);
     __syncthreads();
-    for (int c = threadIdx.x; c < nc; c += 256) wt[c] = kvp::ex2(ml[ch.slot(rc.chunk(c0 + c))].x - ms);
+    for (int c = threadIdx.x; c < nc; c += 256) wt[c] = kvp::ex2(ml[j.ch.slot(j.rc.chunk(c0 + c))].x - ms);
     __syncthreads();
-    // the group's chunks: those with chunk index = grp mod NG, in order
-    for (int r = 0; r < 2; r++) {
-      // the always-visible chunks, then the window's
-      const int lo = max(c0, r ? rc.firsts : 0), hi = min(c0 + nc, r ? rc.count : rc.firsts);
-      if (lo >= hi) continue;
-      const int first = rc.chunk(lo);
-#pragma unroll 4
-      for (int c = lo + ((grp - first % NG + NG) % NG); c < hi; c += NG) {
-        const int sl = ch.slot(rc.chunk(c));
-        const float w = wt[c - c0];
-        const float4 x = *reinterpret_cast<const float4*>(part + (int64_t)sl * HD);
-        acc.x = fmaf(w, x.x, acc.x);
-        acc.y = fmaf(w, x.y, acc.y);
-        acc.z = fmaf(w, x.z, acc.z);
-        acc.w = fmaf(w, x.w, acc.w);
-        sum = fmaf(w, ml[sl].y, sum);
-      }
-    }
+    join_group<N>(j, a.slots, a.part, a.ml, HD, lane, grp, c0, c0 + nc, [&](int c) { return wt[c - c0]; }, acc, sum);
   }
-  os[grp][d4] = acc;
-  if (d4 == 0) sums[grp] = sum;
+#pragma unroll
+  for (int k = 0; k < N; k++) os[grp][lane * N + k] = acc[k];
+  if (lane == 0) sums[grp] = sum;
   __syncthreads();
   if (grp) return;
-  for (int k = 1; k < NG; k++) {
-    const float4 x = os[k][d4];
-    acc.x += x.x;
-    acc.y += x.y;
-    acc.z += x.z;
-    acc.w += x.w;
-    sum += sums[k];
+  sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < N; k++) acc[k] = 0.f;
+  for (int g = 0; g < kGroups; g++) {
+#pragma unroll
+    for (int k = 0; k < N; k++) acc[k] += os[g][lane * N + k];
+    sum += sums[g];
   }
   const float f = sum != 0.f ? __fdiv_rn(1.f, sum) : 0.f;
-  const float x[4] = {acc.x * f, acc.y * f, acc.z * f, acc.w * f};
-  store_n<T, 4>(static_cast<T*>(a.out.p) + (int64_t)row * a.out.row + (int64_t)h * a.out.head + 4 * d4, vec, x);
+#pragma unroll
+  for (int k = 0; k < N; k++) acc[k] *= f;
+  store_n<T, N>(static_cast<T*>(a.out.p) + (int64_t)row * a.out.row + (int64_t)h * a.out.head + lane * N, vec, acc);
 }
 
 template <int HD, int FMT, int NT, bool F32Q>
@@ -596,8 +652,11 @@ bool strides_ok(const KvTensor& t, int item, int bytes) {
 
 template <class T, int HD>
 cudaError_t launch_join(const KvAttnArgs& a, int tq, cudaStream_t st) {
-  return launch_pdl(kv_join_kernel<T, HD>, dim3((unsigned)((int64_t)a.b.rows * a.heads)), dim3(256), 0, st, true, a, tq,
-                    strides_ok(a.out, sizeof(T), 4 * sizeof(T)));
+  const int64_t items = (int64_t)a.b.rows * a.heads;
+  const bool vec = strides_ok(a.out, sizeof(T), 16);
+  if (a.slots <= kFewSlots)
+    return launch_pdl(kv_join_few_kernel<T, HD>, dim3((unsigned)ceil_div(items, 8)), dim3(256), 0, st, true, a, tq, vec);
+  return launch_pdl(kv_join_kernel<T, HD>, dim3((unsigned)items), dim3(256), 0, st, true, a, tq, vec);
 }
 
 }  // namespace

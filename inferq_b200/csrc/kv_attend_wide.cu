@@ -59,22 +59,25 @@ template <int HD, int FMT, bool F32Q>
 struct Geo {
   static constexpr int kTileBytes = kT * HD * 2;  // an f16 tile of keys or values
   static constexpr int kQlo = F32Q ? kM * HD * 2 : 0;
-  static constexpr int kRing = HD < 256 ? 4 : FMT == kKvI8 || F32Q ? 2 : 3;
-  // i8 tiles pass through stages of bytes, for keys and for values each: whole
-  // tiles, but for f32 rows at hd 256, whose second parts leave room for three
-  // quarters of one
+  // Tiles of keys and of values.  f32 rows at hd 256 leave less room: with i8
+  // one tile of values (it is filled again under the next scores' product).
   static constexpr bool kSmall = F32Q && HD == 256;
-  static constexpr int kStageTokens = kSmall ? 16 : kT;
+  static constexpr int kRing = HD < 256 ? 4 : FMT == kKvI8 || F32Q ? 2 : 3;
+  static constexpr int kRingV = kSmall && FMT == kKvI8 ? 1 : kRing;
+  // i8 tiles pass through stages of bytes, for keys and for values each: whole
+  // tiles, or three halves
+  static constexpr int kStageTokens = kSmall ? 32 : kT;
   static constexpr int kStage = FMT == kKvI8 ? kStageTokens * HD : 0;
   static constexpr int kStages = FMT != kKvI8 ? 1 : kSmall || HD < 256 ? 3 : 2;
   static constexpr int kScaleBytes = kScaleRing * (2 * kT + 4) * 4 + 6 * kM * 4;
-  static constexpr int kSmem = 2 * kRing * kTileBytes + kQlo + 2 * kStages * kStage + kScaleBytes + 1024;
+  static constexpr int kSmem = (kRing + kRingV) * kTileBytes + kQlo + 2 * kStages * kStage + kScaleBytes + 1024;
   static constexpr int kExpandWarps = FMT == kKvI8 ? 8 : 0;
   static constexpr int kThreads = (kExpandWarp + kExpandWarps) * 32;
   static constexpr uint32_t kTmemS = HD, kTmemQ = HD + 2 * kT;
   static constexpr uint32_t kTmemCols = HD + 2 * kT + HD / 2 > 256 ? 512 : 256;
   static_assert(HD + 2 * kT + HD / 2 <= 512, "O, S and Q fit the tensor memory");
-  static_assert(kRing * kTileBytes >= kM * HD * 2, "Q is staged where V tiles come later");
+  static_assert((FMT == kKvI8 ? kRing : kRingV) * kTileBytes >= kM * HD * 2, "Q is staged where tiles come later");
+  static_assert(kStages >= (kStageTokens == kT ? 2 : 3) || FMT != kKvI8, "see the loader's turns");
   static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
 };
 
@@ -187,6 +190,15 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // Barrier of a group's two warps (64 threads) that share a quarter of the
 // rows, and whether any of them sets `x`; of all softmax warps.
 __device__ __forceinline__ void pair_sync(int q) { asm volatile("barrier.cta.sync %0, 64;" ::"r"(q + 1) : "memory"); }
+__device__ __forceinline__ bool soft_any(bool x) {
+  uint32_t r;
+  asm volatile(
+      "{ .reg .pred p, c; setp.ne.u32 c, %1, 0; barrier.cta.red.or.pred p, 9, %2, c; selp.u32 %0, 1, 0, p; }"
+      : "=r"(r)
+      : "r"((uint32_t)x), "n"(kSoftWarps * 32)
+      : "memory");
+  return r != 0;
+}
 __device__ __forceinline__ void soft_sync() { asm volatile("barrier.cta.sync 9, %0;" ::"n"(kSoftWarps * 32) : "memory"); }
 __device__ __forceinline__ bool pair_any(int q, bool x) {
   uint32_t r;
@@ -208,8 +220,8 @@ template <int HD, int FMT, bool F32Q>
 __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
     kv_attend_wide_kernel(const __grid_constant__ KvAttnArgs a, const bool vec) {
   using G_ = Geo<HD, FMT, F32Q>;
-  constexpr int R = G_::kRing, TB = G_::kTileBytes, NS = G_::kStages, SB = G_::kStage;
-  __shared__ __align__(8) uint64_t kfull[R], kempty[R], vfull[R], vempty[R], sfull[2], pfull[2], odone, qfull, decided, drained;
+  constexpr int R = G_::kRing, RV = G_::kRingV, TB = G_::kTileBytes, NS = G_::kStages, SB = G_::kStage;
+  __shared__ __align__(8) uint64_t kfull[R], kempty[R], vfull[RV], vempty[RV], sfull[2], pfull[2], odone, qfull, decided, drained;
   __shared__ __align__(8) uint64_t scfull[kScaleRing], scempty[kScaleRing];
   __shared__ __align__(8) uint64_t stfull[2 * NS], stempty[2 * NS];  // stages of keys, then of values
   __shared__ uint32_t tmem_s;
@@ -218,7 +230,10 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
   uint8_t* smem = smem_raw + ((1024 - (su32(smem_raw) & 1023)) & 1023);
   uint8_t* kring = smem;
   uint8_t* vring = smem + R * TB;
-  uint8_t* qlo = vring + R * TB;
+  uint8_t* qlo = vring + RV * TB;
+  // Q's first parts pass through a ring before its tiles come: f16 tiles of
+  // values are needed last, i8 tiles of keys are expanded behind their bytes
+  uint8_t* qring = FMT == kKvI8 ? kring : vring;
   uint8_t* stages = qlo + G_::kQlo;                                 // [keys, values][stage]
   float* scales = reinterpret_cast<float*>(stages + 2 * NS * SB);  // [ring][keys 64, values 64, exponent, pad]
   float* tops = scales + kScaleRing * (2 * kT + 4);  // [half][row] maxima of a tile
@@ -242,6 +257,8 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
     for (int s = 0; s < R; s++) {
       bar_init(&kfull[s], FMT == kKvI8 ? 4 : 1);
       bar_init(&kempty[s], 1);
+    }
+    for (int s = 0; s < RV; s++) {
       bar_init(&vfull[s], FMT == kKvI8 ? 4 : 1);
       bar_init(&vempty[s], 1);
     }
@@ -291,12 +308,13 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
 
   if (warp < kSoftWarps) {
     // ------------------------------------------------------- query rows
-    // Row by row with the lanes along the head; first parts go through the V
+    // Row by row with the lanes along the head; first parts go through a
     // ring (chunks XOR-ed with the row) to the thread that owns the row.
     const int quarter = warp & 3, half = (warp >> 2) & 1, grp = warp >> 3, r0 = quarter * 32;
     const int pair = grp * 4 + quarter, part = warp >> 2;
     {
       constexpr int N = HD / 32, U = 4;  // rows in flight
+#pragma unroll 1  // (straight-line code that runs once costs its instruction fetch)
       for (int rb = 8 * part; rb < 8 * part + 8; rb += U) {
         float x[U][N];
 #pragma unroll
@@ -330,7 +348,7 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
             lo[j] = __float2half_rn(y - __half2float(hi[j]));
           }
           const int byte = lane * N * 2, c = byte >> 4;
-          uint8_t* d = vring + row * HD * 2 + ((c ^ (row & 7)) << 4) + (byte & 15);
+          uint8_t* d = qring + row * HD * 2 + ((c ^ (row & 7)) << 4) + (byte & 15);
           uint8_t* dl = qlo + ((c >> 3) * kM + row) * 128 + (((c & 7) ^ (row & 7)) << 4) + (byte & 15);
           if constexpr (N == 8) {
             *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(hi);
@@ -360,7 +378,7 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
       uint32_t v[8];
 #pragma unroll
       for (int k = 0; k < 2; k++) {
-        const uint4 w = *reinterpret_cast<const uint4*>(vring + row * HD * 2 + (((part * kQC + c + k) ^ (row & 7)) << 4));
+        const uint4 w = *reinterpret_cast<const uint4*>(qring + row * HD * 2 + (((part * kQC + c + k) ^ (row & 7)) << 4));
         v[4 * k] = w.x, v[4 * k + 1] = w.y, v[4 * k + 2] = w.z, v[4 * k + 3] = w.w;
       }
       tmem_st8(lanes + G_::kTmemQ + 4 * (part * kQC + c), v);
@@ -527,16 +545,21 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
     soft_sync();
     float* ls = half ? sums : tops;  // [group][row]
     ls[grp * kM + row] = l2.x + l2.y;
-    soft_sync();
-    if (ok && !__any_sync(0xffffffffu, *abort_v)) {
+    if (!soft_any(!ok || *abort_v)) {  // one outcome for all: barriers follow
       tc_after();
       const float l = (tops[row] + tops[kM + row]) + (sums[row] + sums[kM + row]);
       const int grow = tr.row0 + rr / group, h = kvh * group + rr % group;
       const int64_t rh = (int64_t)grow * a.heads + h;
       const float f = a.slots > 1 ? 1.f : l != 0.f ? __fdiv_rn(1.f, l) : 0.f;
       if (a.slots > 1 && live && part == 0) a.ml[rh * a.slots + slot] = make_float2(m - 7.f + (float)ev, l);
-      auto put = [&](auto* dst, bool v16) {
-        using T = std::remove_reference_t<decltype(*dst)>;
+      // A row's elements lie with one thread: they go to shared memory, a row
+      // of hd elements and 16 bytes apart (so that eight lanes' stores meet
+      // eight bank groups), and from there to memory as whole rows.
+      auto put = [&](auto* base, int64_t at, bool whole_rows) {
+        using T = std::remove_reference_t<decltype(*base)>;
+        constexpr int kRow = HD * (int)sizeof(T) + 16;
+        static_assert(kM * kRow <= (R + RV) * TB + G_::kQlo + 2 * NS * SB, "the rings hold the results");
+        T* mine = reinterpret_cast<T*>(smem + row * kRow);
 #pragma unroll 1
         for (int c = part * (HD / 4); c < (part + 1) * (HD / 4); c += 16) {
           uint32_t o[16];
@@ -546,21 +569,37 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
 #pragma unroll
             for (int j = 0; j < 16; j++) o[j] = 0;
           }
-          if (!live) continue;
 #pragma unroll
           for (int j = 0; j < 16; j += 8) {
             float y[8];
 #pragma unroll
             for (int k = 0; k < 8; k++) y[k] = __uint_as_float(o[j + k]) * f;
-            store_n<T, 8>(dst + c + j, v16, y);
+            store_n<T, 8>(mine + c + j, true, y);
+          }
+        }
+        if (whole_rows) async_fence();
+        // the quarter's four warps hold parts of its rows
+        asm volatile("barrier.cta.sync %0, 128;" ::"r"(10 + quarter) : "memory");
+        if (whole_rows) {
+          if (part == 0 && live)
+            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(base + at), "r"(su32(mine)),
+                         "r"(HD * (int)sizeof(T))
+                         : "memory");
+          asm volatile("cp.async.bulk.commit_group;\ncp.async.bulk.wait_group 0;" ::: "memory");
+        } else {
+          for (int i = 8 * part; i < 8 * part + 8; i++) {
+            const int64_t to = __shfl_sync(0xffffffffu, at, i);
+            if (tr.r0 + r0 + i >= tr.nr) continue;
+            const T* src = reinterpret_cast<const T*>(smem + (r0 + i) * kRow);
+            for (int c = lane; c < HD; c += 32) base[to + c] = src[c];
           }
         }
       };
       const int64_t at = (int64_t)grow * a.out.row + (int64_t)h * a.out.head;
-      if (a.slots > 1) put(a.part + (rh * a.slots + slot) * HD, true);
-      else if constexpr (F32Q) put(static_cast<float*>(a.out.p) + at, vec);
-      else if (a.dtype == F16) put(static_cast<__half*>(a.out.p) + at, vec);
-      else put(static_cast<__nv_bfloat16*>(a.out.p) + at, vec);
+      if (a.slots > 1) put(a.part, (rh * a.slots + slot) * HD, true);
+      else if constexpr (F32Q) put(static_cast<float*>(a.out.p), at, vec);
+      else if (a.dtype == F16) put(static_cast<__half*>(a.out.p), at, vec);
+      else put(static_cast<__nv_bfloat16*>(a.out.p), at, vec);
     }
   } else if (warp == kMmaWarp) {
     // --------------------------------------------------------- products
@@ -597,8 +636,8 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
     for (; ok && ti < sp.end; it++) {
       ti = sp.next(ti);
       if (ti < sp.end && !(ok = score(it + 1))) break;
-      const int s = it % R;
-      ok = wait(&pfull[it & 1], (it >> 1) & 1) && wait(&vfull[s], (it / R) & 1);
+      const int s = it % RV;
+      ok = wait(&pfull[it & 1], (it >> 1) & 1) && wait(&vfull[s], (it / RV) & 1);
       if (!ok) break;
       tc_after();
       if (leader) {
@@ -655,19 +694,19 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
         sv[h] = spool[at * p.page_tokens + ((ti * kT + t) & (p.page_tokens - 1))];
       }
     };
-    // (Turns need a warp to know, from the fill it waited for last, that a
-    // barrier is at most one phase behind the one it waits for.  Two tiles
-    // apart that holds for rings of whole tiles, which are emptied in order; in
-    // a ring of three quarter tiles it does not: one warp fills those.)
-    constexpr bool kTurns = !(FMT == kKvI8 && G_::kSmall);
-    auto after = [&](int ti) { return kTurns ? sp.next(sp.next(ti)) : sp.next(ti); };
-    int it = turn, ti = !turn ? sp.first : kTurns ? sp.next(sp.first) : sp.end, t1 = after(ti);
+    // A parity tells two phases apart only while the barrier is known to be at
+    // most one behind.  Fill n waits for the emptying of fill n - NS, so fill
+    // n - 2 NS has to be known as emptied from the warp's fill before: with
+    // whole tiles n - 2 (behind n - 2 - NS), with halves n - 3 (behind n - 3 -
+    // NS), and the rings are emptied in order: NS >= 2, and >= 3 for halves.
+    auto after = [&](int ti) { return sp.next(sp.next(ti)); };
+    int it = turn, ti = turn ? sp.next(sp.first) : sp.first, t1 = after(ti);
     bool ok = true;
     int page = page_of(ti, ask(ti)), id1 = ask(t1);
     if (ti < sp.end) load_scales(ti, page);
     if (FMT == kKvF16 && isv && ti < sp.end) ok = wait(&qfull, 0);  // the V ring holds the query rows first
     int requested = 0;  // one past the last fill of the ring (f16) or of the stages (i8)
-    for (; ok && ti < sp.end; it += kTurns ? 2 : 1) {
+    for (; ok && ti < sp.end; it += 2) {
       // the tile's scales and the exponent above the values'
       const int sr = it % kScaleRing;
       if (it >= kScaleRing && !(ok = wait(&scempty[sr], ((it / kScaleRing) + 1) & 1))) break;
@@ -706,7 +745,7 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
         __syncwarp();
       } else {
         constexpr int kPer = kT / G_::kStageTokens;  // stages of a tile
-        const int cs = min(rs, G_::kSmall ? 4 : 6), ct = 1 << cs, copies = G_::kStageTokens >> cs;
+        const int cs = min(rs, G_::kSmall ? 5 : 6), ct = 1 << cs, copies = G_::kStageTokens >> cs;
 #pragma unroll 1
         for (int q = 0; q < kPer; q++) {
           const int n = it * kPer + q, s = n % NS;
@@ -742,15 +781,16 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
     uint8_t* ring = isv ? vring : kring;
     uint64_t* full = isv ? vfull : kfull;
     uint64_t* empty = isv ? vempty : kempty;
+    const int rn = isv ? RV : R;
     constexpr int C = HD / 16, TP = 128 / C;         // chunks a token, tokens a pass
     constexpr int kPer = kT / G_::kStageTokens, NP = G_::kStageTokens / TP;  // stages a tile, passes a stage
     const int ch = tid % C, tk = tid / C;
     bool ok = true;
-    if (isv && sp.first < sp.end) ok = wait(&qfull, 0);  // the V ring holds the query rows first
+    if (!isv && sp.first < sp.end) ok = wait(&qfull, 0);  // the K ring holds the query rows first
     int it = 0;
     for (int ti = sp.first; ok && ti < sp.end; ti = sp.next(ti), it++) {
-      const int s = it % R;
-      if (it >= R && !(ok = wait(&empty[s], ((it / R) + 1) & 1))) break;
+      const int s = it % rn;
+      if (it >= rn && !(ok = wait(&empty[s], ((it / rn) + 1) & 1))) break;
       uint8_t* dst = ring + s * TB;
 #pragma unroll
       for (int q = 0; q < kPer; q++) {

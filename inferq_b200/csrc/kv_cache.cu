@@ -199,6 +199,40 @@ cudaError_t kv_read_launch(const KvPool& p, const KvBatch& b, int dtype, const K
   return by_type(false, p, b, dtype, k, v, st);
 }
 
+int kv_create(int format, int kv_heads, int head_dim, int page_tokens, int64_t pages, int* flag, iq_kv& c) {
+  IQ_CUDA(cudaGetDevice(&c.device));
+  // (below 2^31 * 2^8 heads * 2^17 bytes: no overflow)
+  const size_t bytes = (size_t)pages * kv_heads * (size_t)kv_head_bytes(format, head_dim, page_tokens);
+  const size_t sbytes = (size_t)pages * kv_heads * page_tokens * 4;
+  DevBuf* bufs[] = {&c.k, &c.v, &c.ks, &c.vs, &c.flag};
+  const size_t sizes[] = {bytes, bytes, sbytes, sbytes, sizeof(int)};
+  const int n = flag ? 4 : 5;
+  for (int i = 0; i < n; i++) {
+    const cudaError_t e = bufs[i]->reserve(sizes[i]);
+    if (e == cudaErrorMemoryAllocation) cudaGetLastError();  // not sticky: clear it
+    IQ_CHECK(e != cudaErrorMemoryAllocation, IQ_ENOMEM, "no room for a cache of %lld pages (%zu bytes)",
+             (long long)pages, 2 * (bytes + sbytes));
+    IQ_CUDA(e);
+  }
+  // Every token of the pool is finite from the start: kernels may read
+  // tokens of a page that are not written yet, with weight zero.
+  for (int i = 0; i < n; i++) IQ_CUDA(cudaMemset(bufs[i]->p, 0, sizes[i]));
+  IQ_CUDA(cudaStreamSynchronize(nullptr));
+  KvPool& p = c.pool;
+  p.k = c.k.as<uint8_t>();
+  p.v = c.v.as<uint8_t>();
+  p.ks = c.ks.as<float>();
+  p.vs = c.vs.as<float>();
+  p.flag = flag ? flag : c.flag.as<int>();
+  p.pages = pages;
+  p.nkv = kv_heads;
+  p.hd = head_dim;
+  p.page_tokens = page_tokens;
+  p.page_shift = __builtin_ctz((unsigned)page_tokens);
+  p.format = format;
+  return IQ_OK;
+}
+
 }  // namespace iq
 
 using namespace iq;
@@ -299,35 +333,7 @@ int iq_kv_create(int format, int kv_heads, int head_dim, int page_tokens, int64_
   IQ_CHECK(pages >= 1 && pages < (1ll << 31), IQ_EINVAL, "a pool of %lld pages", (long long)pages);
   std::unique_ptr<iq_kv> c(new (std::nothrow) iq_kv);
   IQ_CHECK(c, IQ_ENOMEM, "out of host memory");
-  IQ_CUDA(cudaGetDevice(&c->device));
-  // (below 2^31 * 2^8 heads * 2^17 bytes: no overflow)
-  const size_t bytes = (size_t)pages * kv_heads * (size_t)kv_head_bytes(format, head_dim, page_tokens);
-  const size_t sbytes = (size_t)pages * kv_heads * page_tokens * 4;
-  DevBuf* bufs[] = {&c->k, &c->v, &c->ks, &c->vs, &c->flag};
-  const size_t sizes[] = {bytes, bytes, sbytes, sbytes, sizeof(int)};
-  for (int i = 0; i < 5; i++) {
-    const cudaError_t e = bufs[i]->reserve(sizes[i]);
-    if (e == cudaErrorMemoryAllocation) cudaGetLastError();  // not sticky: clear it
-    IQ_CHECK(e != cudaErrorMemoryAllocation, IQ_ENOMEM, "no room for a cache of %lld pages (%zu bytes)",
-             (long long)pages, 2 * (bytes + sbytes));
-    IQ_CUDA(e);
-  }
-  // Every token of the pool is finite from the start: kernels may read
-  // tokens of a page that are not written yet, with weight zero.
-  for (int i = 0; i < 5; i++) IQ_CUDA(cudaMemset(bufs[i]->p, 0, sizes[i]));
-  IQ_CUDA(cudaStreamSynchronize(nullptr));
-  KvPool& p = c->pool;
-  p.k = c->k.as<uint8_t>();
-  p.v = c->v.as<uint8_t>();
-  p.ks = c->ks.as<float>();
-  p.vs = c->vs.as<float>();
-  p.flag = c->flag.as<int>();
-  p.pages = pages;
-  p.nkv = kv_heads;
-  p.hd = head_dim;
-  p.page_tokens = page_tokens;
-  p.page_shift = __builtin_ctz((unsigned)page_tokens);
-  p.format = format;
+  if (int rc = kv_create(format, kv_heads, head_dim, page_tokens, pages, nullptr, *c)) return rc;
   *out = c.release();
   return IQ_OK;
 }

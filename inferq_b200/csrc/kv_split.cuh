@@ -15,6 +15,9 @@ namespace iq {
 __host__ __device__ inline int64_t kv_min(int64_t a, int64_t b) { return a < b ? a : b; }
 __host__ __device__ inline int64_t kv_max(int64_t a, int64_t b) { return a > b ? a : b; }
 
+// A position inside 0 .. 2^31 - 1 (divisions stay in 32 bits).
+__host__ __device__ inline int kv_clip(int64_t a) { return (int)kv_min(kv_max(a, 0), 0x7fffffff); }
+
 struct KvTileRows {
   int seq, row0;  // the sequence and its first row
   int r0, nr;     // first query row of the tile and query rows (row x head of the KV head) of the sequence
@@ -80,7 +83,7 @@ __host__ __device__ inline KvChunks kv_chunks(const KvAttnArgs& a, int64_t pa) {
   KvChunks c = {0, 0};
   if (a.window) {
     c.first_chunks = (a.sinks + a.chunk - 1) / a.chunk;
-    c.window0 = (int)kv_max(c.first_chunks, kv_max(pa - a.window + 1, 0) / a.chunk);
+    c.window0 = (int)kv_max(c.first_chunks, kv_clip(pa - a.window + 1) / a.chunk);
   }
   return c;
 }
@@ -95,9 +98,9 @@ __host__ __device__ inline KvRowChunks kv_row_chunks(const KvAttnArgs& a, const 
   const int64_t top = kv_min(pos, cap - 1);
   if (top < 0) return {0, 0, 0};
   KvRowChunks r;
-  const int last = (int)(top / a.chunk);
+  const int last = kv_clip(top) / a.chunk;
   r.firsts = (int)kv_min(ch.first_chunks, last + 1);
-  r.window0 = a.window ? (int)kv_max(ch.first_chunks, kv_max(pos - a.window + 1, 0) / a.chunk) : 0;
+  r.window0 = a.window ? (int)kv_max(ch.first_chunks, kv_clip(pos - a.window + 1) / a.chunk) : 0;
   r.count = r.firsts + (int)kv_max(last - r.window0 + 1, 0);
   return r;
 }
@@ -126,7 +129,7 @@ struct KvSpan {
 __host__ __device__ inline KvSpan kv_span(const KvAttnArgs& a, const KvTileRows& t, int tq, int slot) {
   const int group = a.heads / a.pool.nkv;
   const int64_t cap = (int64_t)a.b.table_cols << a.pool.page_shift;
-  const int64_t pa = t.pos + t.r0 / group, pb = t.pos + (kv_min(t.r0 + tq, t.nr) - 1) / group;
+  const int64_t pa = t.pos + t.r0 / group, pb = t.pos + ((int)kv_min(t.r0 + tq, t.nr) - 1) / group;
   const int64_t top = (1ll << 31) - 1;
   KvSpan s;
   s.pa = (int)kv_max(kv_min(pa, top), -top);
@@ -146,10 +149,11 @@ __host__ __device__ inline KvSpan kv_span(const KvAttnArgs& a, const KvTileRows&
 constexpr int kKvTile = 64;  // tokens a tile
 
 // Query rows of a tile: the fewest of 8, 16, 32, 64 that take a sequence's
-// rows of one KV head at once; above 64 rows the tensor-core kernel's 128.
+// rows of one KV head at once; above 64 rows the tensor-core kernel's 128,
+// unless the call keeps to the other.
 inline int kv_tile_query_rows(const KvAttnArgs& a, int max_rows) {
   const int64_t r = (int64_t)(max_rows ? std::min(max_rows, a.b.rows) : a.b.rows) * (a.heads / a.pool.nkv);
-  return r <= 8 ? 8 : r <= 16 ? 16 : r <= 32 ? 32 : r <= 64 ? 64 : 128;
+  return r <= 8 ? 8 : r <= 16 ? 16 : r <= 32 ? 32 : r <= 64 || a.narrow ? 64 : 128;
 }
 inline int64_t kv_tiles_bound(const KvAttnArgs& a, int tq) {
   const int64_t r = (int64_t)a.b.rows * (a.heads / a.pool.nkv);
@@ -166,12 +170,28 @@ inline size_t kv_plan(KvAttnArgs& a, int max_rows) {
   const int tile_tokens = (tq - 1) / group + 1;
   const int64_t span = a.window ? std::min<int64_t>(cap, (int64_t)a.window + a.sinks + tile_tokens + kKvTile) : cap;
   const int64_t items = kv_tiles_bound(a, tq) * a.pool.nkv;
-  if (!a.chunk) {
+  if (!a.chunk && tq <= 64) {
     // Halve the split until two CTAs an SM have two chunks each to take, or a
     // chunk is two tiles.
     int64_t chunk = std::max<int64_t>(align_up(span, kKvTile), 2 * kKvTile);
     while (chunk > 2 * kKvTile && items * ceil_div(span, chunk) < 4 * 148) chunk = align_up(chunk / 2, kKvTile);
     a.chunk = (int)chunk;
+  } else if (!a.chunk) {
+    // One CTA an SM: the split n with the least waves x (tiles of a CTA + what
+    // a CTA costs besides) + the join of n partial results, in tiles' time
+    // (hd / 256 of about 0.7 us, twice that for f32 rows; a CTA's start and
+    // end cost some 6 us, partial results cross HBM twice).
+    const double tile_us = 0.7 * a.pool.hd / 256 * (a.dtype == F32 ? 2 : 1) + 0.4;
+    const double result_us = (double)a.b.rows * a.heads * a.pool.hd * 8 / 5e6;
+    double best = 0;
+    for (int n = 1; n <= 16; n++) {
+      // (unsplit, a chunk holds all of the table: first tokens and window in one)
+      const int64_t chunk = align_up(n == 1 ? std::max<int64_t>(cap, 1) : ceil_div(span, n), kKvTile);
+      const int64_t slots = n == 1 ? 1 : ceil_div(span, chunk) + (a.window ? 1 + (a.sinks > 0) : 0);
+      const double cost = (double)ceil_div(items * slots, 148) * (ceil_div(ceil_div(span, n), kKvTile) * tile_us + 6) +
+                          (n > 1 ? slots * result_us + 4 : 0);
+      if (n == 1 || cost < best) best = cost, a.chunk = (int)chunk;
+    }
   }
   const int64_t all = std::max<int64_t>(ceil_div(cap, a.chunk), 1);
   a.slots = (int)all;

@@ -115,6 +115,11 @@ struct AttnArgs {
   // rows (Q8_K when hd == 256, Q8_0 when hd % 128 == 0) instead of `out`.
   uint8_t* q8k_out; int q8k_stride;
   uint8_t* q80_out; int q80_stride;
+  // Optional, for a state with a paged cache: prep writes the rows' keys to
+  // kstage [rows][nkv][hd] and no cache; the combine takes the attention's
+  // outputs att [rows][nh][hd] instead of partials.
+  float* kstage;
+  const float* att;
 };
 // Positions per split of the scan.  Chunk c always covers absolute positions
 // [c*kAttnChunk, (c+1)*kAttnChunk), and a row combines its chunks in order, so

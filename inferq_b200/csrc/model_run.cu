@@ -568,6 +568,44 @@ int run_delta(Ctx& x, const Layer& L, const LayerRec& R, int k, int li) {
   return IQ_OK;
 }
 
+}  // namespace
+
+int state_kv_attention(iq_state* s, int fi, const int* pos, int rows, const float* k, const float* v, const float* q,
+                       float* out, bool narrow, DevBuf& ws, bool grow) {
+  const iq_config& c = s->m->cfg;
+  const int64_t hd = c.head_dim, kvd = c.num_key_value_heads * hd, nhd = c.num_attention_heads * hd;
+  KvAttnArgs a = {};
+  a.pool = s->kv[fi]->pool;
+  a.b.table = s->kv_table.as<int32_t>();
+  a.b.position = pos;
+  a.b.table_ld = a.b.table_cols = s->kv_pages;
+  // (a launch that is not captured knows its position: the split goes by it)
+  if (!narrow) a.b.table_cols = (int)ceil_div(s->position + rows, kStatePage);
+  a.b.seqs = 1;
+  a.b.rows = rows;
+  ++s->launch_count;
+  IQ_CUDA(kv_append_launch(a.pool, a.b, F32, KvTensor{const_cast<float*>(k), kvd, hd},
+                           KvTensor{const_cast<float*>(v), kvd, hd}, s->st));
+  a.q = KvTensor{const_cast<float*>(q), nhd, hd};
+  a.out = KvTensor{out, nhd, hd};
+  a.dtype = F32;
+  a.heads = c.num_attention_heads;
+  a.scale_log2e = (float)(1.4426950408889634 / sqrt((double)hd));
+  a.window = s->kv_window;
+  a.sinks = s->kv_window ? s->kv_sinks : 0;
+  a.chunk = narrow ? kStateChunk : 0;
+  a.narrow = narrow;
+  const size_t need = kv_attend_plan(a, rows);
+  if (grow) IQ_CUDA(ws.reserve(need));
+  IQ_CHECK(ws.bytes >= need, IQ_ESTATE, "attention workspace of %zu bytes, %zu are needed", ws.bytes, need);
+  kv_attend_bind(a, ws.p);
+  s->launch_count += a.slots > 1 ? 2 : 1;
+  IQ_CUDA(kv_attend_launch(a, rows, s->st));
+  return IQ_OK;
+}
+
+namespace {
+
 int run_attention(Ctx& x, const Layer& L, const LayerRec& R, int k, int fi) {
   iq_state* s = x.s;
   const iq_config& c = x.c;
@@ -588,8 +626,13 @@ int run_attention(Ctx& x, const Layer& L, const LayerRec& R, int k, int fi) {
   a.vp_ld = a.kp_ld;
   a.q_norm = A.q_norm.p();
   a.k_norm = A.k_norm.p();
-  a.kcache = s->kc[fi].as<float>();
-  a.vcache = s->vc[fi].as<float>();
+  if (s->kv_format) {
+    a.kstage = s->kv_stage.as<float>();
+    a.att = s->kv_att.as<float>();
+  } else {
+    a.kcache = s->kc[fi].as<float>();
+    a.vcache = s->vc[fi].as<float>();
+  }
   a.qbuf = s->qbuf.as<float>();
   a.part = s->part.as<float>();
   a.out = s->attn_out.as<float>();
@@ -617,8 +660,12 @@ int run_attention(Ctx& x, const Layer& L, const LayerRec& R, int k, int fi) {
   ++x.s->launch_count;
   IQ_CUDA(attn_prep_launch(a, x.st, x.pdl));
   x.mark("attn.prep");
-  ++x.s->launch_count;
-  IQ_CUDA(attn_scan_launch(a, x.st, x.pdl));
+  if (s->kv_format) {
+    TRY(state_kv_attention(s, fi, a.pos, k, a.kstage, a.vp, a.qbuf, s->kv_att.as<float>(), true, s->kv_ws, false));
+  } else {
+    ++x.s->launch_count;
+    IQ_CUDA(attn_scan_launch(a, x.st, x.pdl));
+  }
   x.mark("attn.scan");
   ++x.s->launch_count;
   IQ_CUDA(attn_combine_launch(a, x.st, x.pdl));
@@ -688,6 +735,8 @@ int run_pass(iq_state* s, int k, bool verify) {
   IQ_CUDA(cudaMemcpyAsync(s->h_result, x.result(), 4 * sizeof(int), cudaMemcpyDeviceToHost, x.st));
   // the GEMVs' bounded-wait status travels back with the result
   if (int* f = qmv_timeout_flag()) IQ_CUDA(cudaMemcpyAsync(s->h_result + 4, f, sizeof(int), cudaMemcpyDeviceToHost, x.st));
+  if (s->kv_format)
+    IQ_CUDA(cudaMemcpyAsync(s->h_result + 5, s->kv_flag.p, sizeof(int), cudaMemcpyDeviceToHost, x.st));
   return IQ_OK;
 }
 
@@ -928,7 +977,38 @@ int alloc_state(iq_state* s) {
     IQ_CUDA(s->dn_layers.reserve(dl.size() * sizeof(DeltaNetLayer)));
     IQ_CUDA(cudaMemcpy(s->dn_layers.p, dl.data(), dl.size() * sizeof(DeltaNetLayer), cudaMemcpyHostToDevice));
   }
-  s->kc.resize(m->n_full + (m->has_mtp ? 1 : 0));
+  const int n_kv = m->n_full + (m->has_mtp ? 1 : 0);
+  if (s->kv_format) {
+    s->kv_pages = (int)ceil_div(s->max_pos + kMaxK, kStatePage);
+    IQ_CUDA(s->kv_flag.reserve(sizeof(int)));
+    IQ_CUDA(cudaMemset(s->kv_flag.p, 0, sizeof(int)));
+    std::vector<int32_t> ids((size_t)s->kv_pages);
+    for (int i = 0; i < s->kv_pages; i++) ids[i] = i;
+    IQ_CUDA(s->kv_table.reserve(ids.size() * 4));
+    IQ_CUDA(cudaMemcpy(s->kv_table.p, ids.data(), ids.size() * 4, cudaMemcpyHostToDevice));
+    for (int i = 0; i < n_kv; i++) {
+      s->kv.emplace_back(new iq_kv);
+      TRY(kv_create(s->kv_format, c.num_key_value_heads, c.head_dim, kStatePage, s->kv_pages, s->kv_flag.as<int>(),
+                    *s->kv.back()));
+    }
+    IQ_CUDA(s->kv_stage.reserve(K * kvd * 4));
+    IQ_CUDA(s->kv_att.reserve(K * nhd * 4));
+    // the workspace of every pass of up to 8 rows, before any is captured
+    KvAttnArgs a = {};
+    a.pool = s->kv.empty() ? KvPool{} : s->kv[0]->pool;
+    a.b.table_cols = s->kv_pages;
+    a.b.seqs = 1;
+    a.heads = c.num_attention_heads;
+    a.window = s->kv_window;
+    a.sinks = s->kv_window ? s->kv_sinks : 0;
+    a.narrow = true;
+    for (int k = 1; n_kv && k <= K; k++) {
+      a.b.rows = k;
+      a.chunk = kStateChunk;
+      IQ_CUDA(s->kv_ws.reserve(kv_attend_plan(a, k)));
+    }
+  }
+  s->kc.resize(s->kv_format ? 0 : n_kv);
   s->vc.resize(s->kc.size());
   for (size_t i = 0; i < s->kc.size(); i++) {
     IQ_CUDA(s->kc[i].reserve((size_t)(align_up(s->max_pos + kMaxK, kAttnChunk) * kvd * 4)));
@@ -949,7 +1029,8 @@ int alloc_state(iq_state* s) {
   IQ_CUDA(s->qbuf.reserve(K * nhd * 4));
   IQ_CUDA(s->attn_out.reserve(K * nhd * 4));
   s->max_chunks = (int)ceil_div(s->max_pos + kMaxK, kAttnChunk);
-  IQ_CUDA(s->part.reserve((size_t)K * c.num_attention_heads * s->max_chunks * (c.head_dim + 2) * 4));
+  if (!s->kv_format)
+    IQ_CUDA(s->part.reserve((size_t)K * c.num_attention_heads * s->max_chunks * (c.head_dim + 2) * 4));
   const int64_t slots = K * topk + K;
   IQ_CUDA(s->logits_moe.reserve(K * (E + 1) * 4));
   IQ_CUDA(s->route_e.reserve((c.num_hidden_layers + 1) * K * topk * 4));
@@ -982,6 +1063,14 @@ int alloc_state(iq_state* s) {
 // After a synchronized pass: a GEMV that gave up waiting for its weights
 // (bounded wait) fails the call with IQ_ETIMEDOUT; the flag is cleared.
 int check_device_waits(iq_state* s) {
+  if (s->h_result[5]) {
+    const int f = s->h_result[5];
+    s->h_result[5] = 0;
+    IQ_CUDA(cudaMemset(s->kv_flag.p, 0, sizeof(int)));
+    IQ_CHECK(!(f & kKvTimeout), IQ_ETIMEDOUT,
+             "attention over the cache gave up a bounded device wait; results of this pass are invalid");
+    IQ_CHECK(!f, IQ_ESTATE, "a row stood outside the state's cache");
+  }
   if (!s->h_result[4]) return IQ_OK;
   s->h_result[4] = 0;
   if (int* f = qmv_timeout_flag()) IQ_CUDA(cudaMemset(f, 0, sizeof(int)));
@@ -1022,13 +1111,31 @@ using namespace iq;
 extern "C" {
 
 int iq_state_create(iq_model* m, int64_t max_positions, iq_state** out) {
+  return iq_state_create_kv(m, max_positions, IQ_F32, 0, 0, out);
+}
+
+int iq_state_create_kv(iq_model* m, int64_t max_positions, int kv_format, int window, int sinks, iq_state** out) {
   clear_error();
   IQ_CHECK(m && out, IQ_EINVAL, "iq_state_create: null argument");
+  IQ_CHECK(kv_format == IQ_F32 || kv_format == IQ_F16 || kv_format == IQ_I8, IQ_EUNSUPPORTED,
+           "unsupported cache format %d; expected F32 (%d), F16 (%d) or I8 (%d)", kv_format, IQ_F32, IQ_F16, IQ_I8);
+  IQ_CHECK(window >= 0 && sinks >= 0, IQ_EINVAL, "window %d and sinks %d cannot be negative", window, sinks);
+  IQ_CHECK(kv_format != IQ_F32 || window == 0, IQ_EUNSUPPORTED, "a window needs an F16 or I8 cache");
+  const iq_config& c = m->cfg;
+  IQ_CHECK(kv_format == IQ_F32 ||
+               ((c.head_dim == 64 || c.head_dim == 128 || c.head_dim == 256) && c.num_key_value_heads <= 256 &&
+                c.num_attention_heads % c.num_key_value_heads == 0 &&
+                c.num_attention_heads / c.num_key_value_heads <= 128),
+           IQ_EUNSUPPORTED, "no F16 or I8 cache for %d heads over %d KV heads of %d elements", c.num_attention_heads,
+           c.num_key_value_heads, c.head_dim);
   IQ_CHECK(max_positions > 0 && max_positions <= m->cfg.max_position_embeddings, IQ_EINVAL,
            "max_positions %lld outside 1..%d", (long long)max_positions, m->cfg.max_position_embeddings);
   std::unique_ptr<iq_state> s(new iq_state);
   s->m = m;
   s->max_pos = max_positions;
+  s->kv_format = kv_format;
+  s->kv_window = window;
+  s->kv_sinks = sinks;
   int rc = alloc_state(s.get());
   if (rc) return rc;
   rc = reset_state(s.get());
@@ -1089,6 +1196,51 @@ int64_t image_bytes(const iq_state* s, const StateImageHeader& h) {
   if (h.has_mtp) b += 2 * h.mtp_position * h.kv_dim * 4;
   return b;
 }
+// KV rows 0 .. position - 1 of cache fi as the image keeps them, [pos][kv_head][hd]
+// f32, keys then values: out of (to_host) or into the state.  A paged cache's
+// rows pass through device buffers of up to 4096 rows.
+int image_kv_rows(iq_state* s, int fi, int64_t position, uint8_t* p, bool to_host) {
+  const iq_config& c = s->m->cfg;
+  const int64_t kvd = (int64_t)c.num_key_value_heads * c.head_dim;
+  const size_t n = (size_t)position * kvd * 4;
+  if (!s->kv_format) {
+    for (int v = 0; v < 2; v++) {
+      void* dev = v ? s->vc[fi].p : s->kc[fi].p;
+      if (to_host) IQ_CUDA(cudaMemcpy(p + v * n, dev, n, cudaMemcpyDeviceToHost));
+      else IQ_CUDA(cudaMemcpy(dev, p + v * n, n, cudaMemcpyHostToDevice));
+    }
+    return IQ_OK;
+  }
+  const int64_t most = std::min<int64_t>(position, 4096);
+  const size_t half = (size_t)most * kvd * 4;
+  IQ_CUDA(s->kv_rows.reserve(2 * half + 16));
+  uint8_t* k = s->kv_rows.as<uint8_t>();
+  int32_t* at = reinterpret_cast<int32_t*>(k + 2 * half);
+  for (int64_t r0 = 0; r0 < position; r0 += most) {
+    const int64_t rows = std::min(most, position - r0);
+    const size_t bytes = (size_t)rows * kvd * 4, off = (size_t)r0 * kvd * 4;
+    const int32_t first = (int32_t)r0;
+    IQ_CUDA(cudaMemcpyAsync(at, &first, sizeof first, cudaMemcpyHostToDevice, s->st));
+    KvBatch b = {};
+    b.table = s->kv_table.as<int32_t>();
+    b.position = at;
+    b.table_ld = b.table_cols = s->kv_pages;
+    b.seqs = 1;
+    b.rows = (int)rows;
+    const KvTensor kt = {k, kvd, c.head_dim}, vt = {k + half, kvd, c.head_dim};
+    if (!to_host) {
+      IQ_CUDA(cudaMemcpyAsync(k, p + off, bytes, cudaMemcpyHostToDevice, s->st));
+      IQ_CUDA(cudaMemcpyAsync(k + half, p + n + off, bytes, cudaMemcpyHostToDevice, s->st));
+      IQ_CUDA(kv_append_launch(s->kv[fi]->pool, b, F32, kt, vt, s->st));
+    } else {
+      IQ_CUDA(kv_read_launch(s->kv[fi]->pool, b, F32, kt, vt, s->st));
+      IQ_CUDA(cudaMemcpyAsync(p + off, k, bytes, cudaMemcpyDeviceToHost, s->st));
+      IQ_CUDA(cudaMemcpyAsync(p + n + off, k + half, bytes, cudaMemcpyDeviceToHost, s->st));
+    }
+    IQ_CUDA(cudaStreamSynchronize(s->st));
+  }
+  return IQ_OK;
+}
 }  // namespace
 
 int iq_state_image_size(const iq_state* s, int64_t* bytes) {
@@ -1119,8 +1271,7 @@ int iq_state_export(iq_state* s, void* out, int64_t bytes) {
   for (const Layer& L : s->m->layers) {
     if (L.type == kFull) {
       const size_t n = (size_t)h.position * h.kv_dim * 4;
-      IQ_CUDA(cudaMemcpy(p, s->kc[fi].p, n, cudaMemcpyDeviceToHost));
-      IQ_CUDA(cudaMemcpy(p + n, s->vc[fi].p, n, cudaMemcpyDeviceToHost));
+      TRY(image_kv_rows(s, fi, h.position, p, true));
       p += 2 * n;
       fi++;
     } else {
@@ -1152,11 +1303,7 @@ int iq_state_export(iq_state* s, void* out, int64_t bytes) {
       li++;
     }
   }
-  if (h.has_mtp) {
-    const size_t n = (size_t)h.mtp_position * h.kv_dim * 4;
-    IQ_CUDA(cudaMemcpy(p, s->kc[s->m->n_full].p, n, cudaMemcpyDeviceToHost));
-    IQ_CUDA(cudaMemcpy(p + n, s->vc[s->m->n_full].p, n, cudaMemcpyDeviceToHost));
-  }
+  if (h.has_mtp) TRY(image_kv_rows(s, s->m->n_full, h.mtp_position, p, true));
   return IQ_OK;
 }
 
@@ -1184,8 +1331,7 @@ int iq_state_import(iq_state* s, const void* in, int64_t bytes) {
   for (const Layer& L : s->m->layers) {
     if (L.type == kFull) {
       const size_t n = (size_t)h.position * h.kv_dim * 4;
-      IQ_CUDA(cudaMemcpy(s->kc[fi].p, p, n, cudaMemcpyHostToDevice));
-      IQ_CUDA(cudaMemcpy(s->vc[fi].p, p + n, n, cudaMemcpyHostToDevice));
+      TRY(image_kv_rows(s, fi, h.position, const_cast<uint8_t*>(p), false));
       p += 2 * n;
       fi++;
     } else {
@@ -1196,11 +1342,7 @@ int iq_state_import(iq_state* s, const void* in, int64_t bytes) {
       li++;
     }
   }
-  if (h.has_mtp) {
-    const size_t n = (size_t)h.mtp_position * h.kv_dim * 4;
-    IQ_CUDA(cudaMemcpy(s->kc[s->m->n_full].p, p, n, cudaMemcpyHostToDevice));
-    IQ_CUDA(cudaMemcpy(s->vc[s->m->n_full].p, p + n, n, cudaMemcpyHostToDevice));
-  }
+  if (h.has_mtp) TRY(image_kv_rows(s, s->m->n_full, h.mtp_position, const_cast<uint8_t*>(p), false));
   // the imported DeltaNet state is conv ring slot 0 and the recurrent base
   // with no records pending; positions from the header
   int ctrl[8] = {(int)h.position, 0, 0, 0, 0, (int)h.mtp_position, 0, 0};
@@ -1208,6 +1350,16 @@ int iq_state_import(iq_state* s, const void* in, int64_t bytes) {
   s->position = h.position;
   s->mtp_position = h.mtp_position;
   s->can_rollback = false;
+  return IQ_OK;
+}
+
+int iq_state_kv_bytes(const iq_state* s, int64_t* bytes) {
+  IQ_CHECK(s && bytes, IQ_EINVAL, "iq_state_kv_bytes: null argument");
+  int64_t b = 0;
+  for (auto& x : s->kc) b += (int64_t)x.bytes;
+  for (auto& x : s->vc) b += (int64_t)x.bytes;
+  for (auto& x : s->kv) b += (int64_t)(x->k.bytes + x->v.bytes + x->ks.bytes + x->vs.bytes);
+  *bytes = b;
   return IQ_OK;
 }
 
@@ -1243,6 +1395,7 @@ int iq_forward(iq_state* s, const uint32_t* tokens, int rows, float* logits, flo
       if (wflag) IQ_CUDA(cudaMemset(f, 0, sizeof(int)));
     }
     if (int* f = qmv_timeout_flag()) IQ_CUDA(cudaMemcpy(s->h_result + 4, f, sizeof(int), cudaMemcpyDeviceToHost));
+    if (s->kv_format) IQ_CUDA(cudaMemcpy(s->h_result + 5, s->kv_flag.p, sizeof(int), cudaMemcpyDeviceToHost));
     TRY(check_device_waits(s));
     IQ_CHECK(!wflag, IQ_ETIMEDOUT, "a wide product gave up a bounded device wait; results of this call are invalid");
     s->can_rollback = true;

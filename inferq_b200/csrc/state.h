@@ -2,8 +2,10 @@
 // model_run.cu and the wide prefill pass in wide_pass.cu).
 #pragma once
 #include <map>
+#include <memory>
 #include <string>
 #include <vector>
+#include "kv.h"
 #include "model.h"
 
 namespace iq {
@@ -31,6 +33,10 @@ struct KPlan {
 };
 
 constexpr int kMaxDraft = 16;  // MTP draft steps per call
+// Tokens per attention split over a paged cache.  Fixed, so that a row of a
+// pass of up to 8 rows depends on its own context only.
+constexpr int kStateChunk = 256;
+constexpr int kStatePage = 64;
 
 }  // namespace iq
 
@@ -52,8 +58,13 @@ struct iq_state {
   std::vector<iq::DevBuf> rec, rec_log;  // per linear layer: base state, update records
   std::vector<iq::DevBuf> dn_qkv, dn_ba;  // per linear layer pass projections
   iq::DevBuf dn_layers;  // DeltaNetLayer[n_linear]
-  // attention
+  // attention: f32 rows [pos][kv_head][hd], or (kv_format) a paged cache a
+  // layer with one block table 0, 1, 2, ..
   std::vector<iq::DevBuf> kc, vc;
+  int kv_format = 0, kv_window = 0, kv_sinks = 0;
+  std::vector<std::unique_ptr<iq_kv>> kv;
+  int kv_pages = 0;
+  iq::DevBuf kv_table, kv_flag, kv_ws, kv_stage, kv_att, kv_rows;
   // scratch
   iq::DevBuf hidden, xn, act8k, act80, z, dn_out, qg, kp, vp, qbuf, part, attn_out;
   iq::DevBuf logits_moe, route_e, route_w, gu_jobs, down_jobs, counts, union_list, gu_out, act_mid, y;
@@ -86,7 +97,7 @@ struct iq_state {
   // the wide prefill pass's buffers (allocated on its first use)
   struct Wide {
     iq::DevBuf hidden, xn, big, z, ba, o, y, kp, vp, logits, tokens, ctrl, lg, re, rw, xg, actg, gu, yg, ysh, gush,
-        map, jobs, argres, scratch, qbuf, part, cv, bl, dno, wyx, wym, wyew, yslot;
+        map, jobs, argres, scratch, qbuf, part, kstage, att, kvws, cv, bl, dno, wyx, wym, wyew, yslot;
     int attn_rows = 8;  // rows per attention slice of the chunk
     int32_t* h_routes = nullptr;  // pinned [rows][topk]
     std::vector<iq::QmvJob> job_table;
@@ -115,6 +126,11 @@ struct iq_state {
 
 
 namespace iq {
+// Rows of layer fi's paged cache at *pos, *pos + 1, .. (device): written from
+// k, v [rows][kv_head][hd] f32 and attended to by q [rows][head][hd] f32.
+// `ws` grows as needed where `grow` is set (never under capture).
+int state_kv_attention(iq_state* s, int fi, const int* pos, int rows, const float* k, const float* v, const float* q,
+                       float* out, bool narrow, DevBuf& ws, bool grow);
 // The wide prefill pass (wide_pass.cu): `rows` tokens at the state's
 // position through every layer in chunks of kWideRows; outputs as iq_forward.
 constexpr int kWideRows = 512;

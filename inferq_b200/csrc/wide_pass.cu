@@ -280,6 +280,36 @@ int wide_attention(iq_state* s, const Layer& L, int fi, int n) {
   TRY_IQ(wide_project(s, A.q, W.xn.as<float>(), c.hidden_size, n, W.big.as<float>(), 2 * nhd));
   TRY_IQ(wide_project(s, A.k, W.xn.as<float>(), c.hidden_size, n, W.kp.as<float>(), kvd));
   TRY_IQ(wide_project(s, A.v, W.xn.as<float>(), c.hidden_size, n, W.vp.as<float>(), kvd));
+  if (s->kv_format) {
+    // a paged cache: the chunk's rows enter it and attend to it in one launch each
+    AttnArgs a = {};
+    a.qg = W.big.as<float>();
+    a.qg_ld = 2 * nhd;
+    a.kp = W.kp.as<float>();
+    a.kp_ld = kvd;
+    a.vp = W.vp.as<float>();
+    a.vp_ld = kvd;
+    a.q_norm = A.q_norm.p();
+    a.k_norm = A.k_norm.p();
+    a.kstage = W.kstage.as<float>();
+    a.qbuf = W.qbuf.as<float>();
+    a.att = W.att.as<float>();
+    a.out = W.o.as<float>();
+    a.out_ld = nhd;
+    a.rows = n;
+    a.nh = c.num_attention_heads;
+    a.nkv = c.num_key_value_heads;
+    a.hd = c.head_dim;
+    a.rotary_dim = c.rotary_dim;
+    a.theta = c.rope_theta;
+    a.eps = c.rms_norm_eps;
+    a.pos = W.ctrl.as<int>() + 2;
+    IQ_CUDA(attn_prep_launch(a, s->st, false));
+    TRY_IQ(state_kv_attention(s, fi, a.pos, n, a.kstage, a.vp, a.qbuf, W.att.as<float>(), false, W.kvws, true));
+    IQ_CUDA(attn_combine_launch(a, s->st, false));
+    TRY_IQ(wide_project(s, A.o, W.o.as<float>(), nhd, n, W.y.as<float>(), c.hidden_size));
+    return add_rows(s, W.hidden.as<float>(), W.y.as<float>(), (int64_t)n * c.hidden_size);
+  }
   // slices of W.attn_rows rows: every row's arithmetic is its own (fixed
   // 32-position chunks merged in order), so the slice size changes no result
   const int R = W.attn_rows;
@@ -519,7 +549,11 @@ int alloc_wide(iq_state* s, int n) {
   IQ_CUDA(W.vp.reserve(n * kvd * 4));
   IQ_CUDA(W.tokens.reserve(n * 4));
   IQ_CUDA(W.ctrl.reserve((2 + ceil_div(n, 8)) * 4));
-  if (c.num_attention_heads > 0 && s->m->n_linear < c.num_hidden_layers) {
+  if (s->kv_format) {
+    IQ_CUDA(W.qbuf.reserve(n * nhd * 4));
+    IQ_CUDA(W.kstage.reserve(n * kvd * 4));
+    IQ_CUDA(W.att.reserve(n * nhd * 4));
+  } else if (c.num_attention_heads > 0 && s->m->n_linear < c.num_hidden_layers) {
     // attention slices: as many rows as the scan's shared memory and a
     // partials buffer of at most 512 MB hold
     AttnArgs g = {};

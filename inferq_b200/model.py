@@ -43,6 +43,9 @@ def _declare(L):
         "iq_model_destroy": (None, [P]),
         "iq_model_weight_bytes": (ctypes.c_int, [P, ctypes.POINTER(ctypes.c_int64)]),
         "iq_state_create": (ctypes.c_int, [P, ctypes.c_int64, ctypes.POINTER(P)]),
+        "iq_state_create_kv": (ctypes.c_int, [P, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                             ctypes.POINTER(P)]),
+        "iq_state_kv_bytes": (ctypes.c_int, [P, ctypes.POINTER(ctypes.c_int64)]),
         "iq_state_destroy": (None, [P]),
         "iq_state_reset": (ctypes.c_int, [P]),
         "iq_state_position": (ctypes.c_int, [P, ctypes.POINTER(ctypes.c_int64)]),
@@ -133,13 +136,26 @@ class Model:
 
 
 class State:
-    """Decode state (KV cache + DeltaNet state) of one sequence."""
+    """Decode state (KV cache + DeltaNet state) of one sequence.  ``kv``: the
+    cache's format, "f32" rows as the reference keeps them or a paged cache of
+    "f16" or "i8" vectors; with one of these a ``window`` limits attention to
+    the last positions and the first ``sinks``."""
 
-    def __init__(self, model: Model, max_positions: int):
+    KV_FORMATS = {"f32": 0, "f16": 1, "i8": 24}
+
+    def __init__(self, model: Model, max_positions: int, *, kv: str = "f32", window: int = 0, sinks: int = 0):
+        if kv not in self.KV_FORMATS:
+            raise ValueError(f"KV cache format {kv!r}; expected one of {sorted(self.KV_FORMATS)}")
         self.model = model
         h = P()
-        _lib.check(lib().iq_state_create(model._h, max_positions, ctypes.byref(h)))
+        _lib.check(lib().iq_state_create_kv(model._h, max_positions, self.KV_FORMATS[kv], window, sinks, ctypes.byref(h)))
         self._h = h
+
+    @property
+    def kv_bytes(self) -> int:
+        v = ctypes.c_int64()
+        _lib.check(lib().iq_state_kv_bytes(self._h, ctypes.byref(v)))
+        return v.value
 
     @property
     def position(self) -> int:
