@@ -58,6 +58,7 @@ struct KvAttnArgs {
   float scale_log2e;   // score scale times log2(e)
   int window, sinks;   // window 0: none
   int chunk;           // tokens per split, a multiple of 64
+  int tq;              // query rows a tile: 8, 16, 32, 64 or the tensor-core kernel's 128
   int slots;           // splits that a tile of query rows can need
   bool narrow;         // never the tensor-core kernel (its rows' results depend on the launch)
   float* part;         // slots > 1: [row][head][slot][hd] unnormalised outputs
@@ -76,12 +77,12 @@ cudaError_t kv_append_launch(const KvPool& p, const KvBatch& b, int dtype, const
 cudaError_t kv_read_launch(const KvPool& p, const KvBatch& b, int dtype, const KvTensor& k, const KvTensor& v,
                            cudaStream_t st);
 
-// The split of an attention call: fills chunk and slots (chunk 0 on entry:
+// The split of an attention call: fills tq, chunk and slots (chunk 0 on entry:
 // chosen here) and returns the workspace bytes it needs (0 when unsplit).
 size_t kv_attend_plan(KvAttnArgs& a, int max_rows);
 // a.part / a.ml point into the workspace.
 void kv_attend_bind(KvAttnArgs& a, void* workspace);
-cudaError_t kv_attend_launch(const KvAttnArgs& a, int max_rows, cudaStream_t st);
+cudaError_t kv_attend_launch(const KvAttnArgs& a, cudaStream_t st);
 
 }  // namespace iq
 

@@ -100,19 +100,14 @@ __device__ __forceinline__ float2 unpack2(uint32_t w) { return __half22float2(*r
 
 template <int HD, int FMT, int NT, bool F32Q>
 struct Geo {
-  static constexpr int kElt = FMT == kKvI8 ? 1 : 2;
-  static constexpr int kTileBytes = kTile * HD * kElt;  // of keys, and of values
+  static constexpr KvNarrow kGeo = kv_narrow(FMT, HD, NT, F32Q);
+  static constexpr int kTileBytes = kTile * HD * (FMT == kKvI8 ? 1 : 2);  // of keys, and of values
   static constexpr int kTQ = 8 * NT;
-  static constexpr int kQld = HD * 2 + 16;              // bytes of a staged query row
+  static constexpr int kQld = HD * 2 + 16;                                // bytes of a staged query row
   static constexpr int kQBytes = kTQ * kQld * (F32Q ? 2 : 1);
   static constexpr int kPBytes = NT * 4 * 32 * 8 * (F32Q ? 2 : 1);
-  static constexpr int kFixed = kQBytes + kPBytes + 4 * kTQ * 4 + 2 * kTQ * 4 + 64;
-  // Stages: two CTAs on an SM where a stage is at most 32 KB, up to four
-  // stages of small tiles; a stage's 512 bytes of scales are counted in.
-  static constexpr int kPer = 2 * kTileBytes + 512;
-  static constexpr int kRoom = (2 * kTileBytes <= 32768 && kFixed <= 48 * 1024 ? 112 : 226) * 1024 - 2048 - kFixed;
-  static constexpr int kStages = kRoom / kPer > 4 ? 4 : kRoom / kPer;
-  static constexpr int kSmem = kStages * kPer + kFixed + 1024;
+  static_assert(kGeo.fixed == kQBytes + kPBytes + 6 * kTQ * 4 + 64, "queries, weights, maxima, factors, positions");
+  static constexpr int kStages = kGeo.stages, kSmem = kGeo.smem;
   static_assert(kStages >= 2, "two stages keep a copy in flight");
 };
 
@@ -512,89 +507,109 @@ struct JoinRow {
 };
 // False for a row behind the last sequence.  Warp-wide.
 __device__ __forceinline__ bool join_row(const KvAttnArgs& a, int row, int h, int tq, int lane, JoinRow* j) {
-  int i;
-  const int seq = kv_seq_of_row(a.b, row, lane, &i);
-  if (seq < 0) return false;
+  const KvSeq q = kv_seq_of_row(a.b, row, lane);
+  if (q.seq < 0) return false;
   const int group = a.heads / a.pool.nkv;
-  const int64_t base = a.b.position[seq];
-  const int tile0 = (i * group + h % group) / tq * tq;  // the row's tile begins here
-  j->ch = kv_chunks(a, base + tile0 / group);
-  j->rc = kv_row_chunks(a, j->ch, base + i);
+  const int tile0 = (q.in_seq * group + h % group) / tq * tq;  // the row's tile begins here
+  j->ch = kv_chunks(a, q.pos + tile0 / group);
+  j->rc = kv_row_chunks(a, j->ch, q.pos + q.in_seq);
   j->rh = (int64_t)row * a.heads + h;
   return true;
 }
-// acc and sum of the group's chunks lo .. hi - 1 of the row (weights w(c)).
-template <int N, class W>
-__device__ __forceinline__ void join_group(const JoinRow& j, int slots, const float* part, const float2* ml, int hd,
-                                           int lane, int g, int lo, int hi, W weight, float (&acc)[N], float& sum) {
-  for (int r = 0; r < 2; r++) {  // the always-visible chunks, then the window's
-    const int b = max(lo, r ? j.rc.firsts : 0), e = min(hi, r ? j.rc.count : j.rc.firsts);
-    if (b >= e) continue;
-    const int first = j.rc.chunk(b);
-#pragma unroll 2
-    for (int c = b + ((g - first) & (kGroups - 1)); c < e; c += kGroups) {
-      const int64_t at = j.rh * slots + j.ch.slot(j.rc.chunk(c));
-      const float w = weight(c);
-      float x[N];
-      load_n<float, N>(part + at * hd + lane * N, true, x);
-#pragma unroll
-      for (int k = 0; k < N; k++) acc[k] = fmaf(w, x[k], acc[k]);
-      sum = fmaf(w, ml[at].y, sum);
-    }
-  }
+// Chunks [b, e) are a run of one of the row's two lists (first tokens, window).
+struct JoinRun {
+  int b, e;
+};
+__device__ __forceinline__ JoinRun join_run(const JoinRow& j, int r) {
+  if (r == 0) return {0, j.rc.firsts};
+  return {j.rc.window0, j.rc.window0 + j.rc.count - j.rc.firsts};
 }
 
-// Up to 32 slots: one warp per (row, head).
+// One warp per (row, head), for many of those: the chunks in blocks of eight,
+// one to a group, all of a block's loads in flight at once.
 template <class T, int HD>
-__global__ void __launch_bounds__(256) kv_join_few_kernel(const __grid_constant__ KvAttnArgs a, const int tq,
+__global__ void __launch_bounds__(128) kv_join_few_kernel(const __grid_constant__ KvAttnArgs a, const int tq,
                                                           const bool vec) {
   constexpr int N = HD / 32;
   pdl_wait();
   const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int row = (int)(item / a.heads), h = (int)(item % a.heads);
   if (row >= a.b.rows) return;
   JoinRow j;
   if (!join_row(a, row, h, tq, lane, &j)) return;
-  const float m = lane < j.rc.count ? a.ml[j.rh * a.slots + j.ch.slot(j.rc.chunk(lane))].x : -INFINITY;
-  float M = m;
+  const float2* ml = a.ml + j.rh * a.slots;
+  const float* part = a.part + j.rh * a.slots * HD + lane * N;
+  const float2 mine = lane < j.rc.count ? ml[j.ch.slot(j.rc.chunk(lane))] : make_float2(-INFINITY, 0.f);
+  float M = mine.x;
 #pragma unroll
   for (int w = 16; w; w >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, w));
-  const float wt = kvp::ex2(m - (M == -INFINITY ? 0.f : M));
-  float acc[N], sum = 0.f;
+  const float wt = kvp::ex2(mine.x - (M == -INFINITY ? 0.f : M));
+  float acc[kGroups][N], sums[kGroups];
 #pragma unroll
-  for (int k = 0; k < N; k++) acc[k] = 0.f;
-#pragma unroll 1
   for (int g = 0; g < kGroups; g++) {
-    float x[N], s = 0.f;
+    sums[g] = 0.f;
 #pragma unroll
-    for (int k = 0; k < N; k++) x[k] = 0.f;
-    join_group<N>(j, a.slots, a.part, a.ml, HD, lane, g, 0, j.rc.count,
-                  [&](int c) { return __shfl_sync(0xffffffffu, wt, c); }, x, s);
+    for (int k = 0; k < N; k++) acc[g][k] = 0.f;
+  }
+#pragma unroll 1
+  for (int r = 0; r < 2; r++) {
+    const JoinRun run = join_run(j, r);
+    const int at = (r ? j.rc.firsts : 0) - run.b;  // a chunk's place among the row's
+#pragma unroll 1
+    for (int c0 = run.b & ~(kGroups - 1); c0 < run.e; c0 += kGroups) {
+      float x[kGroups][N];
 #pragma unroll
-    for (int k = 0; k < N; k++) acc[k] += x[k];
-    sum += s;
+      for (int g = 0; g < kGroups; g++)
+        if (c0 + g >= run.b && c0 + g < run.e) load_n<float, N>(part + (int64_t)j.ch.slot(c0 + g) * HD, true, x[g]);
+#pragma unroll
+      for (int g = 0; g < kGroups; g++) {
+        const float w = __shfl_sync(0xffffffffu, wt, (c0 + g + at) & 31), l = __shfl_sync(0xffffffffu, mine.y, (c0 + g + at) & 31);
+        if (c0 + g < run.b || c0 + g >= run.e) continue;
+#pragma unroll
+        for (int k = 0; k < N; k++) acc[g][k] = fmaf(w, x[g][k], acc[g][k]);
+        sums[g] = fmaf(w, l, sums[g]);
+      }
+    }
+  }
+  float o[N], sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < N; k++) o[k] = 0.f;
+#pragma unroll
+  for (int g = 0; g < kGroups; g++) {
+#pragma unroll
+    for (int k = 0; k < N; k++) o[k] += acc[g][k];
+    sum += sums[g];
   }
   const float f = sum != 0.f ? __fdiv_rn(1.f, sum) : 0.f;
 #pragma unroll
-  for (int k = 0; k < N; k++) acc[k] *= f;
-  store_n<T, N>(static_cast<T*>(a.out.p) + (int64_t)row * a.out.row + (int64_t)h * a.out.head + lane * N, vec, acc);
+  for (int k = 0; k < N; k++) o[k] *= f;
+  store_n<T, N>(static_cast<T*>(a.out.p) + (int64_t)row * a.out.row + (int64_t)h * a.out.head + lane * N, vec, o);
 }
 
-// Any number of slots: one CTA per (row, head), a warp per group.
+// One CTA per (row, head), a warp per group, any number of slots.
 template <class T, int HD>
 __global__ void __launch_bounds__(256) kv_join_kernel(const __grid_constant__ KvAttnArgs a, const int tq,
                                                       const bool vec) {
-  constexpr int N = HD / 32, kWeights = 1024;
-  __shared__ float wt[kWeights], red[8], sums[kGroups], os[kGroups][HD];
+  constexpr int N = HD / 32, kWeights = 1024, U = 8;
+  __shared__ float2 wt[kWeights];  // {weight, sum}
+  __shared__ float red[8], sums[kGroups], os[kGroups][HD];
   pdl_wait();
   const int row = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
   const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
   JoinRow j;
   if (!join_row(a, row, h, tq, lane, &j)) return;
   const float2* ml = a.ml + j.rh * a.slots;
+  const float* part = a.part + j.rh * a.slots * HD + lane * N;
   float mxv = -INFINITY;
-  for (int c = threadIdx.x; c < j.rc.count; c += 256) mxv = fmaxf(mxv, ml[j.ch.slot(j.rc.chunk(c))].x);
+  float2 held[kWeights / 256];
+#pragma unroll
+  for (int i = 0; i < kWeights / 256; i++) {
+    const int c = threadIdx.x + 256 * i;
+    held[i] = c < j.rc.count ? ml[j.ch.slot(j.rc.chunk(c))] : make_float2(-INFINITY, 0.f);
+    mxv = fmaxf(mxv, held[i].x);
+  }
+  for (int c = kWeights + threadIdx.x; c < j.rc.count; c += 256) mxv = fmaxf(mxv, ml[j.ch.slot(j.rc.chunk(c))].x);
 #pragma unroll
   for (int w = 16; w; w >>= 1) mxv = fmaxf(mxv, __shfl_xor_sync(0xffffffffu, mxv, w));
   if (lane == 0) red[grp] = mxv;
@@ -606,12 +621,38 @@ __global__ void __launch_bounds__(256) kv_join_kernel(const __grid_constant__ Kv
   float acc[N], sum = 0.f;
 #pragma unroll
   for (int k = 0; k < N; k++) acc[k] = 0.f;
-  for (int c0 = 0; c0 < j.rc.count; c0 += kWeights) {
-    const int nc = min(kWeights, j.rc.count - c0);
+  for (int p0 = 0; p0 < j.rc.count; p0 += kWeights) {  // places p0 .. p0 + 1023 of the row's chunks
+    const int p1 = min(p0 + kWeights, j.rc.count);
     __syncthreads();
-    for (int c = threadIdx.x; c < nc; c += 256) wt[c] = kvp::ex2(ml[j.ch.slot(j.rc.chunk(c0 + c))].x - ms);
+#pragma unroll
+    for (int i = 0; i < kWeights / 256; i++) {
+      const int c = p0 + threadIdx.x + 256 * i;
+      if (c >= p1) continue;
+      const float2 v = p0 ? ml[j.ch.slot(j.rc.chunk(c))] : held[i];
+      wt[c - p0] = make_float2(kvp::ex2(v.x - ms), v.y);
+    }
     __syncthreads();
-    join_group<N>(j, a.slots, a.part, a.ml, HD, lane, grp, c0, c0 + nc, [&](int c) { return wt[c - c0]; }, acc, sum);
+    for (int r = 0; r < 2; r++) {
+      JoinRun run = join_run(j, r);
+      const int at = (r ? j.rc.firsts : 0) - run.b;
+      run.b = max(run.b, p0 - at);
+      run.e = min(run.e, p1 - at);
+      // the group's chunks of the run, eight loads in flight
+      for (int c0 = run.b + ((grp - run.b) & (kGroups - 1)); c0 < run.e; c0 += U * kGroups) {
+        float x[U][N];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+          if (c0 + u * kGroups < run.e) load_n<float, N>(part + (int64_t)j.ch.slot(c0 + u * kGroups) * HD, true, x[u]);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+          if (c0 + u * kGroups >= run.e) continue;
+          const float2 w = wt[c0 + u * kGroups + at - p0];
+#pragma unroll
+          for (int k = 0; k < N; k++) acc[k] = fmaf(w.x, x[u][k], acc[k]);
+          sum = fmaf(w.x, w.y, sum);
+        }
+      }
+    }
   }
 #pragma unroll
   for (int k = 0; k < N; k++) os[grp][lane * N + k] = acc[k];
@@ -654,8 +695,10 @@ template <class T, int HD>
 cudaError_t launch_join(const KvAttnArgs& a, int tq, cudaStream_t st) {
   const int64_t items = (int64_t)a.b.rows * a.heads;
   const bool vec = strides_ok(a.out, sizeof(T), 16);
-  if (a.slots <= kFewSlots)
-    return launch_pdl(kv_join_few_kernel<T, HD>, dim3((unsigned)ceil_div(items, 8)), dim3(256), 0, st, true, a, tq, vec);
+  // a warp each where there are warps enough for the GPU (8 an SM), or little
+  // to join
+  if (a.slots <= kFewSlots && (items >= 8 * 148 || a.slots <= kGroups))
+    return launch_pdl(kv_join_few_kernel<T, HD>, dim3((unsigned)ceil_div(items, 4)), dim3(128), 0, st, true, a, tq, vec);
   return launch_pdl(kv_join_kernel<T, HD>, dim3((unsigned)items), dim3(256), 0, st, true, a, tq, vec);
 }
 
@@ -669,8 +712,8 @@ void kv_attend_bind(KvAttnArgs& a, void* workspace) {
   a.ml = reinterpret_cast<float2*>(a.part + (int64_t)a.b.rows * a.heads * a.slots * a.pool.hd);
 }
 
-cudaError_t kv_attend_launch(const KvAttnArgs& a, int max_rows, cudaStream_t st) {
-  const int tq = kv_tile_query_rows(a, max_rows);
+cudaError_t kv_attend_launch(const KvAttnArgs& a, cudaStream_t st) {
+  const int tq = a.tq;
   const int64_t ctas = kv_tiles_bound(a, tq) * a.pool.nkv * a.slots;
   if (ctas >= (1ll << 31)) return cudaErrorInvalidValue;
   const int item = a.dtype == F32 ? 4 : 2;

@@ -12,11 +12,17 @@
 // it and no others (a zero weight never meets a NaN element).
 //
 // The code is the rounding of the real quotient, not of a float one: the f32
-// quotient (three roundings of 2^-24, so at most 127 * 3 * 2^-24 < 2^-15 off)
-// decides except within 2^-15 of a border between two codes, where 64 bits
-// decide: 127 x is exact there, and a quotient of 24-bit numbers that is no
-// tie is further from one than the division rounds.  So a code depends on
-// nothing but x and amax.
+// product x * (127 / amax) (two roundings of 2^-24, so at most 127 * 2^-23 <
+// 2^-15 off) decides except within 2^-15 of a border between two codes, where
+// 64 bits decide: 127 x is exact there, and a quotient of 24-bit numbers that
+// is no tie is further from one than the division rounds.  So a code depends
+// on nothing but x and amax.
+//
+// What bounds both kernels.  The bytes, if the instructions allow: a warp's
+// 32 bytes in and out a lane come with some 4 instructions an element, so the
+// arithmetic is written for few of them (rounding and byte by one addition of
+// 1.5 * 2^23 + 128, two f32 an operation, one test for all of a lane's
+// borders), and a row's place is found by one thread, not by its warp.
 #include <cmath>
 #include <memory>
 #include <new>
@@ -26,127 +32,216 @@
 namespace iq {
 namespace {
 
-__device__ __forceinline__ int code_i8(float x, float inv, float amax) {
-  const float v = x * 127.f * inv;
-  const float r = rintf(v);
-  if (0.5f - fabsf(v - r) < 0x1p-15f) return (int)rint(127.0 * (double)x / (double)amax);
-  return (int)r;
+constexpr float kMagic = 12582912.f + 128.f;  // v + kMagic holds rint(v) + 128 in its low byte, |v| <= 127
+
+__device__ __forceinline__ float max_nan_abs(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(fabsf(a)), "f"(fabsf(b)));
+  return d;
+}
+// Low bytes of four words.
+__device__ __forceinline__ uint32_t low_bytes(float a, float b, float c, float d) {
+  const uint32_t x = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040);
+  const uint32_t y = __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040);
+  return __byte_perm(x, y, 0x5410);
 }
 
-// One warp per (row, KV head) for keys and values together: 2 x hd elements
-// in, quantised in registers, out as 16-byte chunks or parts of them.  The
-// work is the bytes (hd = 256, f32 rows: 2 KB in, 0.5 KB out a warp).
-template <class T, int HD, int FMT>
-__global__ void __launch_bounds__(256) kv_append_kernel(KvPool p, KvBatch b, KvTensor k, KvTensor v, bool vec) {
-  constexpr int N = HD / 32;
-  const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int row = (int)(item / p.nkv), head = (int)(item % p.nkv);
-  if (row >= b.rows) return;
-  float x[2][N];
-  load_n<T, N>(static_cast<const T*>(k.p) + row * k.row + head * k.head + lane * N, vec, x[0]);
-  load_n<T, N>(static_cast<const T*>(v.p) + row * v.row + head * v.head + lane * N, vec, x[1]);
-  int i;
-  const int s = kv_seq_of_row(b, row, lane, &i);
-  if (s < 0) return;
-  const int64_t pos = (int64_t)b.position[s] + i;
-  if (pos < 0) return;
-  const int page = kv_page(p, b, s, pos);
-  if (page < 0) return;
-  const int t = (int)pos & (p.page_tokens - 1);
-  const int64_t run = (int64_t)page * p.nkv + head;
+// (A call: inlined sixteen times it does not fit the instruction cache.)
+__device__ __noinline__ float code_f64(float x, float amax) {
+  return (float)rint(127.0 * (double)x / (double)amax) + kMagic;
+}
+
+// Biased codes of N elements; amax finite and above zero.  kShort: x and amax
+// have at most 11 significant bits (f16 and bf16 rows).  A quotient 127 x /
+// amax that is no tie then lies at least 2^-20 of itself from one ((254 mx 2^k
+// - (2n + 1) ma) / 2 ma is a multiple of 2^k / 2 ma with ma < 2^11 and 2^k >=
+// q / 254), and the f32 product is within 2^-23: what lies within 2^-21 of a
+// border is a tie, and goes to the even side.  16-bit rows meet ties in up to
+// 40% of their vectors.
+template <int N, bool kShort>
+__device__ __forceinline__ void codes_i8(const float (&x)[N], float amax, uint8_t* out) {
+  float far = 0.f, t[N], d[N];
+  const bool middle = amax > 0x1p-100f && amax < 0x1p100f;  // else the factor or a product leaves f32's normals
+  const float c = middle ? __fdiv_rn(127.f, amax) : 0.f;
 #pragma unroll
-  for (int w = 0; w < 2; w++) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int j = 0; j < N; j++) m = max(m, __float_as_uint(x[w][j]) & 0x7fffffffu);
-    m = __reduce_max_sync(0xffffffffu, m);
-    const bool finite = m < 0x7f800000u;
-    const float amax = __uint_as_float(m);
-    float scale;
-    uint8_t* dst = (w ? p.v : p.k) + run * kv_head_bytes(FMT, HD, p.page_tokens);
-    if constexpr (FMT == kKvI8) {
-      // both sides of the quotient moved by 2^64, away from f32's ends (an x
-      // that falls below the normals there is below amax / 2^62: code 0)
-      const float f = amax >= 1.f ? 0x1p-64f : 0x1p64f;
-      const float am = amax * f;
-      const bool live = finite && m != 0;
-      const float inv = live ? __fdiv_rn(1.f, am) : 0.f;
-      scale = finite ? __fdiv_rn(amax, 127.f) : __int_as_float(0x7fffffff);
-      alignas(8) uint8_t q[N];
-#pragma unroll
-      for (int j = 0; j < N; j++)
-        q[j] = (uint8_t)((live ? code_i8(x[w][j] * f, inv, am) : 0) + 128);
-      const int c = lane * N;
-      dst += kv_chunk<FMT, HD>(t, c >> 4, p.page_tokens) + (c & 15);
-      if constexpr (N == 8) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(q);
-      else if constexpr (N == 4) *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(q);
-      else *reinterpret_cast<uint16_t*>(dst) = *reinterpret_cast<const uint16_t*>(q);
-    } else {
-      const int e = f16_exponent(amax);
-      scale = finite ? kvp::pow2i(e) : __int_as_float(0x7fffffff);
-      const float f = kvp::pow2i(-e);
-      alignas(16) __half h[N];
-#pragma unroll
-      for (int j = 0; j < N; j++) h[j] = __float2half_rn(finite ? x[w][j] * f : 0.f);
-      const int c = lane * N * 2;
-      dst += kv_chunk<FMT, HD>(t, c >> 4, p.page_tokens) + (c & 15);
-      if constexpr (N == 8) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(h);
-      else if constexpr (N == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(h);
-      else *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(h);
+  for (int j = 0; j < N; j += 2) {
+    const float2 v = kvp::mul2(make_float2(x[j], x[j + 1]), make_float2(c, c));
+    const float2 u = kvp::add2(v, make_float2(kMagic, kMagic));
+    const float2 r = kvp::add2(u, make_float2(-kMagic, -kMagic));
+    const float2 e = kvp::add2(v, make_float2(-r.x, -r.y));
+    t[j] = u.x;
+    t[j + 1] = u.y;
+    d[j] = e.x;
+    d[j + 1] = e.y;
+    far = fmaxf(far, fmaxf(fabsf(e.x), fabsf(e.y)));
+  }
+  constexpr float kNear = 0.5f - 0x1p-15f;
+  if (far > kNear || !middle) {
+#pragma unroll  // (an index that varies would put the arrays in local memory)
+    for (int j = 0; j < N; j++) {
+      if (kShort && middle) {
+        const bool tie = 0.5f - fabsf(d[j]) < fabsf(x[j] * c) * 0x1p-21f;
+        if (tie && (__float_as_uint(t[j]) & 1)) t[j] += copysignf(1.f, d[j]);
+      } else if (fabsf(d[j]) > kNear || !middle) {
+        t[j] = code_f64(x[j], amax);
+      }
     }
-    if (lane == 0) (w ? p.vs : p.ks)[run * p.page_tokens + t] = scale;
+  }
+  if constexpr (N == 2) {
+    *reinterpret_cast<uint16_t*>(out) = (uint16_t)__byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; j += 4)
+      reinterpret_cast<uint32_t*>(out)[j / 4] = low_bytes(t[j], t[j + 1], t[j + 2], t[j + 3]);
   }
 }
 
-// The reverse: one warp per (row, KV head); rows at negative positions or
-// behind the table read as zeros.
-template <class T, int HD, int FMT>
-__global__ void __launch_bounds__(256) kv_read_kernel(KvPool p, KvBatch b, KvTensor k, KvTensor v, bool vec) {
-  constexpr int N = HD / 32;
-  const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int row = (int)(item / p.nkv), head = (int)(item % p.nkv);
-  if (row >= b.rows) return;
-  int i;
-  const int s = kv_seq_of_row(b, row, lane, &i);
-  if (s < 0) return;
-  const int64_t pos = (int64_t)b.position[s] + i;
-  const int page = pos < 0 ? -1 : kv_page(p, b, s, pos);
-  const int t = (int)pos & (p.page_tokens - 1);
-  const int64_t run = (int64_t)page * p.nkv + head;
-  float x[2][N];
-#pragma unroll
-  for (int w = 0; w < 2; w++) {
-    if (page < 0) {
-#pragma unroll
-      for (int j = 0; j < N; j++) x[w][j] = 0.f;
-      continue;
+template <int B>
+__device__ __forceinline__ void copy_bytes(void* dst, const void* src) {
+  if constexpr (B == 16) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
+  else if constexpr (B == 8) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(src);
+  else if constexpr (B == 4) *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(src);
+  else *reinterpret_cast<uint16_t*>(dst) = *reinterpret_cast<const uint16_t*>(src);
+}
+
+// Where the CTA's items (row, KV head) lie, found by one thread each: a page
+// and a token in it, kNoRow behind the last sequence, kPadding at a negative
+// position, -1 outside the table or the pool.
+constexpr int kNoRow = -2, kPadding = -3, kMostItems = 32;
+
+__device__ __forceinline__ int2 place_of(const KvPool& p, const KvBatch& b, int row) {
+  int s = 0, first = 0;
+  if (b.row_start) {
+    int hi = b.seqs;  // the first sequence that ends behind the row
+    while (s < hi) {
+      const int mid = (s + hi) >> 1;
+      if (b.row_start[mid + 1] <= row) s = mid + 1;
+      else hi = mid;
     }
-    const uint8_t* src = (w ? p.v : p.k) + run * kv_head_bytes(FMT, HD, p.page_tokens);
-    const float scale = (w ? p.vs : p.ks)[run * p.page_tokens + t];
-    if constexpr (FMT == kKvI8) {
-      const int c = lane * N;
-      src += kv_chunk<FMT, HD>(t, c >> 4, p.page_tokens) + (c & 15);
-      alignas(8) uint8_t q[N];
-      if constexpr (N == 8) *reinterpret_cast<uint2*>(q) = *reinterpret_cast<const uint2*>(src);
-      else if constexpr (N == 4) *reinterpret_cast<uint32_t*>(q) = *reinterpret_cast<const uint32_t*>(src);
-      else *reinterpret_cast<uint16_t*>(q) = *reinterpret_cast<const uint16_t*>(src);
+    if (s == b.seqs) return make_int2(kNoRow, 0);
+    first = b.row_start[s];
+    if (row < first) return make_int2(kNoRow, 0);
+  }
+  const int64_t pos = (int64_t)b.position[s] + (row - first);
+  if (pos < 0) return make_int2(kPadding, 0);
+  return make_int2(kv_page(p, b, s, pos), (int)pos & (p.page_tokens - 1));
+}
+
+// A CTA takes 8 `turns` items, a warp one in turn: keys and values of a row's
+// head.  Loads are hidden by the SM's other warps: at most 51 registers, five
+// CTAs an SM (with 88, for the next item's loads in registers, two CTAs fitted
+// and 16384 bf16 rows took 37 us).
+template <class T, int HD, int FMT>
+__global__ void __launch_bounds__(256, 5) kv_append_kernel(const __grid_constant__ KvPool p, const __grid_constant__ KvBatch b,
+                                                        KvTensor k, KvTensor v, bool vec, int turns) {
+  constexpr int N = HD / 32;
+  constexpr int kB = FMT == kKvI8 ? N : 2 * N;  // bytes a lane
+  __shared__ int2 places[kMostItems];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t items = (uint32_t)b.rows * p.nkv, item0 = blockIdx.x * 8 * turns;  // (below 2^31: checked by the caller)
+  auto load = [&](uint32_t item, float (&x)[2][N]) {
+    if (item >= items) return;
+    const int64_t row = item / (uint32_t)p.nkv, head = item - (uint32_t)row * p.nkv;
+    load_n<T, N>(static_cast<const T*>(k.p) + row * k.row + head * k.head + lane * N, vec, x[0]);
+    load_n<T, N>(static_cast<const T*>(v.p) + row * v.row + head * v.head + lane * N, vec, x[1]);
+  };
+  float x[2][N];
+  if (turns == 1) load(item0 + warp, x);  // (under the search)
+  if (threadIdx.x < 8 * turns && item0 + threadIdx.x < items)
+    places[threadIdx.x] = place_of(p, b, (int)((item0 + threadIdx.x) / (uint32_t)p.nkv));
+  __syncthreads();
+  for (int turn = 0; turn < turns; turn++) {
+    const uint32_t item = item0 + turn * 8 + warp;
+    if (item >= items) return;
+    if (turns > 1) load(item, x);
+    const int2 at = places[turn * 8 + warp];
+    if (at.x >= 0) {
+      const int64_t run = (int64_t)at.x * p.nkv + item % (uint32_t)p.nkv;
+      const int64_t off = run * kv_head_bytes(FMT, HD, p.page_tokens) +
+                          kv_chunk<FMT, HD>(at.y, lane * kB >> 4, p.page_tokens) + (lane * kB & 15);
 #pragma unroll
-      for (int j = 0; j < N; j++) x[w][j] = (float)((int)q[j] - 128) * scale;
-    } else {
-      const int c = lane * N * 2;
-      src += kv_chunk<FMT, HD>(t, c >> 4, p.page_tokens) + (c & 15);
-      alignas(16) __half h[N];
-      if constexpr (N == 8) *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(src);
-      else if constexpr (N == 4) *reinterpret_cast<uint2*>(h) = *reinterpret_cast<const uint2*>(src);
-      else *reinterpret_cast<uint32_t*>(h) = *reinterpret_cast<const uint32_t*>(src);
+      for (int w = 0; w < 2; w++) {
+        float m = max_nan_abs(x[w][0], x[w][1]);
 #pragma unroll
-      for (int j = 0; j < N; j++) x[w][j] = __half2float(h[j]) * scale;
+        for (int j = 2; j < N; j++) m = max_nan_abs(m, x[w][j]);
+        // as bits a NaN is above every number
+        const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+        const float amax = __uint_as_float(bits);
+        const bool finite = bits < 0x7f800000u;
+        float scale;
+        alignas(16) uint8_t held[kB];
+        if constexpr (FMT == kKvI8) {
+          scale = finite ? __fdiv_rn(amax, 127.f) : __int_as_float(0x7fffffff);
+          if (finite && bits) {
+            codes_i8<N, sizeof(T) == 2>(x[w], amax, held);
+          } else {
+#pragma unroll
+            for (int j = 0; j < N; j++) held[j] = 128;
+          }
+        } else {
+          const int e = f16_exponent(amax);
+          scale = finite ? kvp::pow2i(e) : __int_as_float(0x7fffffff);
+          const float f = kvp::pow2i(-e);
+#pragma unroll
+          for (int j = 0; j < N; j += 2)
+            reinterpret_cast<__half2*>(held)[j / 2] =
+                finite ? __floats2half2_rn(x[w][j] * f, x[w][j + 1] * f) : __floats2half2_rn(0.f, 0.f);
+        }
+        copy_bytes<kB>((w ? p.v : p.k) + off, held);
+        if (lane == 0) (w ? p.vs : p.ks)[run * p.page_tokens + at.y] = scale;
+      }
     }
   }
-  store_n<T, N>(static_cast<T*>(k.p) + row * k.row + head * k.head + lane * N, vec, x[0]);
-  store_n<T, N>(static_cast<T*>(v.p) + row * v.row + head * v.head + lane * N, vec, x[1]);
+}
+
+// The reverse; rows at negative positions or behind the table read as zeros.
+template <class T, int HD, int FMT>
+__global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ KvPool p, const __grid_constant__ KvBatch b,
+                                                      KvTensor k, KvTensor v, bool vec, int turns) {
+  constexpr int N = HD / 32;
+  constexpr int kB = FMT == kKvI8 ? N : 2 * N;
+  __shared__ int2 places[kMostItems];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t items = (uint32_t)b.rows * p.nkv, item0 = blockIdx.x * 8 * turns;
+  if (threadIdx.x < 8 * turns && item0 + threadIdx.x < items)
+    places[threadIdx.x] = place_of(p, b, (int)((item0 + threadIdx.x) / (uint32_t)p.nkv));
+  __syncthreads();
+#pragma unroll 2
+  for (int turn = 0; turn < turns; turn++) {
+    const uint32_t item = item0 + turn * 8 + warp;
+    if (item >= items) return;
+    const int2 at = places[turn * 8 + warp];
+    if (at.x == kNoRow) continue;
+    const int64_t row = item / (uint32_t)p.nkv, head = item - (uint32_t)row * p.nkv, run = (int64_t)at.x * p.nkv + head;
+    const int64_t off = run * kv_head_bytes(FMT, HD, p.page_tokens) +
+                        kv_chunk<FMT, HD>(at.y, lane * kB >> 4, p.page_tokens) + (lane * kB & 15);
+    float x[2][N];
+#pragma unroll
+    for (int w = 0; w < 2; w++) {
+      alignas(16) uint8_t held[kB];
+      float scale = 0.f;
+      if (at.x >= 0) {
+        copy_bytes<kB>(held, (w ? p.v : p.k) + off);
+        scale = (w ? p.vs : p.ks)[run * p.page_tokens + at.y];
+      }
+#pragma unroll
+      for (int j = 0; j < N; j += 2) {
+        float2 f;
+        if constexpr (FMT == kKvI8) {
+          // 2^23 + u as f32, minus 2^23 + 128: the code, exactly
+          f = make_float2(__uint_as_float(0x4b000000u | held[j]), __uint_as_float(0x4b000000u | held[j + 1]));
+          f = kvp::add2(f, make_float2(-8388736.f, -8388736.f));
+        } else {
+          f = __half22float2(reinterpret_cast<const __half2*>(held)[j / 2]);
+        }
+        f = kvp::mul2(f, make_float2(scale, scale));
+        x[w][j] = at.x < 0 ? 0.f : f.x;
+        x[w][j + 1] = at.x < 0 ? 0.f : f.y;
+      }
+    }
+    store_n<T, N>(static_cast<T*>(k.p) + row * k.row + head * k.head + lane * N, vec, x[0]);
+    store_n<T, N>(static_cast<T*>(v.p) + row * v.row + head * v.head + lane * N, vec, x[1]);
+  }
 }
 
 // Whether every lane's elements start on a multiple of their own size (16
@@ -160,11 +255,14 @@ template <class T>
 cudaError_t launch(bool append, const KvPool& p, const KvBatch& b, const KvTensor& k, const KvTensor& v,
                    cudaStream_t st) {
   const bool vec = vector_ok(k, sizeof(T), p.hd) && vector_ok(v, sizeof(T), p.hd);
-  const unsigned grid = (unsigned)ceil_div((int64_t)b.rows * p.nkv, 8);
+  // items a warp: one, until 64 warps an SM have four each
+  const int64_t items = (int64_t)b.rows * p.nkv;
+  const int turns = items >= 4 * 64 * 148 ? kMostItems / 8 : 1;
+  const unsigned grid = (unsigned)ceil_div(items, 8 * turns);
   auto go = [&](auto hd, auto fmt) {
     constexpr int HD = decltype(hd)::value, FMT = decltype(fmt)::value;
-    if (append) kv_append_kernel<T, HD, FMT><<<grid, 256, 0, st>>>(p, b, k, v, vec);
-    else kv_read_kernel<T, HD, FMT><<<grid, 256, 0, st>>>(p, b, k, v, vec);
+    if (append) kv_append_kernel<T, HD, FMT><<<grid, 256, 0, st>>>(p, b, k, v, vec, turns);
+    else kv_read_kernel<T, HD, FMT><<<grid, 256, 0, st>>>(p, b, k, v, vec, turns);
     return cudaGetLastError();
   };
   using I8 = std::integral_constant<int, kKvI8>;
@@ -308,6 +406,8 @@ int rows_call(const char* name, bool append, const iq_kv* c, const iq_kv_batch* 
   if (int rc = check_type(name, dtype)) return rc;
   if (!b.rows || !b.seqs) return IQ_OK;
   const KvPool& p = c->pool;
+  IQ_CHECK((int64_t)b.rows * p.nkv < (1ll << 31) - 8, IQ_EINVAL, "%s: %d rows of %d KV heads are too many", name, b.rows,
+           p.nkv);
   if (int rc = check_tensor(name, "keys", k, b.rows, p.nkv, p.hd, dtype, !append)) return rc;
   if (int rc = check_tensor(name, "values", v, b.rows, p.nkv, p.hd, dtype, !append)) return rc;
   OnDevice on(c->device);
@@ -418,7 +518,7 @@ int iq_kv_attend(const iq_kv* c, const iq_kv_batch* batch, const iq_kv_attn* at,
   kv_attend_bind(a, workspace);
   OnDevice on(c->device);
   IQ_CUDA(on.err);
-  IQ_CUDA(kv_attend_launch(a, batch->max_rows, static_cast<cudaStream_t>(stream)));
+  IQ_CUDA(kv_attend_launch(a, static_cast<cudaStream_t>(stream)));
   return IQ_OK;
 }
 

@@ -7,26 +7,33 @@
 
 namespace iq {
 
-// Sequence of `row` (warp-wide; every lane returns it) and the row's index in
-// it; -1 when the row lies behind the last sequence.  row_start ascends; each
-// round narrows the range 32-fold.
-__device__ __forceinline__ int kv_seq_of_row(const KvBatch& b, int row, int lane, int* in_seq) {
-  if (!b.row_start) {
-    *in_seq = row;
-    return 0;
-  }
+// Sequence of `row` (warp-wide; every lane returns it), the row's index in it,
+// the sequence's rows and its first position; -1 when the row lies behind the
+// last sequence.  row_start ascends; each round narrows the range 32-fold, and
+// the last round's loads are the answer's.
+struct KvSeq {
+  int seq, in_seq, rows;
+  int64_t pos;
+};
+__device__ __forceinline__ KvSeq kv_seq_of_row(const KvBatch& b, int row, int lane) {
+  if (!b.row_start) return {0, row, b.rows, b.position[0]};
   int lo = 0, n = b.seqs;  // the sequences that end at or before `row` number lo .. lo + n
-  while (n > 0) {
+  while (n > 32) {
     const int step = (n + 31) >> 5;
     const int at = lo + (lane + 1) * step;  // row_start[at] ends the lane's group
     const bool before = (lane + 1) * step <= n && b.row_start[at] <= row;
     const int full = __popc(__ballot_sync(0xffffffffu, before));
     lo += full * step;
-    n = step > 1 ? min(step - 1, b.seqs - lo) : 0;
+    n = min(step, b.seqs - lo);
   }
-  if (lo >= b.seqs) return -1;
-  *in_seq = row - b.row_start[lo];
-  return *in_seq < 0 ? -1 : lo;
+  const int s = min(lo + lane, b.seqs - 1);
+  const int begin = b.row_start[s], end = b.row_start[s + 1], pos = b.position[s];
+  const uint32_t past = __ballot_sync(0xffffffffu, lane < n && end > row);
+  if (!past) return {-1, 0, 0, 0};
+  const int at = __ffs(past) - 1;
+  const int first = __shfl_sync(0xffffffffu, begin, at);
+  return {row < first ? -1 : lo + at, row - first, __shfl_sync(0xffffffffu, end, at) - first,
+          __shfl_sync(0xffffffffu, pos, at)};
 }
 
 // Page that holds position `pos` (>= 0) of sequence `s`; -1 (and the pool's

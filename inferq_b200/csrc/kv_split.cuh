@@ -32,20 +32,24 @@ __device__ __forceinline__ bool kv_tile_rows(const KvBatch& b, int tile, int tq,
     t->seq = t->row0 = 0;
     n = b.rows;
     t->r0 = tile * tq;
+    t->pos = b.position[0];
   } else if (group % tq == 0) {  // no tile crosses a row: no sum over sequences
     const int per = group / tq, row = tile / per;
-    int i;
-    t->seq = row < b.rows ? kv_seq_of_row(b, row, lane, &i) : -1;
-    if (t->seq < 0) return false;
-    t->row0 = row - i;
-    n = b.row_start[t->seq + 1] - t->row0;
-    t->r0 = i * group + tile % per * tq;
+    if (row >= b.rows) return false;
+    const KvSeq q = kv_seq_of_row(b, row, lane);
+    if (q.seq < 0) return false;
+    t->seq = q.seq;
+    t->row0 = row - q.in_seq;
+    t->pos = q.pos;
+    n = q.rows;
+    t->r0 = q.in_seq * group + tile % per * tq;
   } else {
     int before = 0;  // tiles of the sequences up to s0
     t->seq = -1;
     for (int s0 = 0; s0 < b.seqs; s0 += 32) {
-      const int s = s0 + lane;
-      const int rows = s < b.seqs ? max(b.row_start[s + 1] - b.row_start[s], 0) : 0;
+      const int s = min(s0 + lane, b.seqs - 1);
+      const int begin = b.row_start[s], end = b.row_start[s + 1], pos = b.position[s];
+      const int rows = s0 + lane < b.seqs ? max(end - begin, 0) : 0;
       const int tiles = (int)(((int64_t)rows * group + tq - 1) / tq);
       int sum = tiles;
 #pragma unroll
@@ -58,17 +62,17 @@ __device__ __forceinline__ bool kv_tile_rows(const KvBatch& b, int tile, int tq,
         const int at = __ffs(past) - 1;
         t->seq = s0 + at;
         t->r0 = (tile - before - __shfl_sync(0xffffffffu, sum - tiles, at)) * tq;
+        t->row0 = __shfl_sync(0xffffffffu, begin, at);
+        t->pos = __shfl_sync(0xffffffffu, pos, at);
+        n = __shfl_sync(0xffffffffu, rows, at);
         break;
       }
       before += __shfl_sync(0xffffffffu, sum, 31);
     }
     if (t->seq < 0) return false;
-    t->row0 = b.row_start[t->seq];
-    n = b.row_start[t->seq + 1] - t->row0;
   }
   if (t->row0 < 0) return false;
   t->nr = min(n, b.rows - t->row0) * group;
-  t->pos = b.position[t->seq];
   return t->r0 < t->nr;
 }
 
@@ -148,12 +152,34 @@ __host__ __device__ inline KvSpan kv_span(const KvAttnArgs& a, const KvTileRows&
 // ------------------------------------------------------------ host side
 constexpr int kKvTile = 64;  // tokens a tile
 
+// Shared memory of the split kernel (kv_attend.cu): 8 nt query rows, tiles of
+// 64 tokens, two to four stages; three CTAs an SM where two stages and the rest
+// take a third of it, else two, else one.
+struct KvNarrow {
+  int fixed, stages, smem, ctas;
+};
+constexpr KvNarrow kv_narrow(int format, int hd, int nt, bool f32) {
+  const int tile = kKvTile * hd * (format == kKvI8 ? 1 : 2), per = 2 * tile + 512, parts = f32 ? 2 : 1;
+  KvNarrow g = {};
+  g.fixed = 8 * nt * (hd * 2 + 16) * parts + nt * 1024 * parts + 6 * 8 * nt * 4 + 64;
+  const int limit = 2 * tile > 32768 ? 226 : g.fixed <= 10 * 1024 ? 78 : g.fixed <= 48 * 1024 ? 112 : 226;
+  const int room = limit * 1024 - 2048 - g.fixed;
+  g.stages = room / per > 4 ? 4 : room / per;
+  g.smem = g.stages * per + g.fixed + 1024;
+  g.ctas = (227 * 1024) / (g.smem + 1280);  // (static shared memory and 1 KB a CTA)
+  return g;
+}
+
 // Query rows of a tile: the fewest of 8, 16, 32, 64 that take a sequence's
-// rows of one KV head at once; above 64 rows the tensor-core kernel's 128,
-// unless the call keeps to the other.
+// rows of one KV head at once, or the tensor-core kernel's 128: above 64 rows
+// unless the call keeps to the other, and above 32 where the split is free
+// too (16 sequences over 4127 tokens, 8 heads to a KV head, f32 and bf16 rows:
+// of 4 rows 59 and 45 us here, 61 and 51 us there; of 8 rows 136 and 113 us
+// here, 65 and 54 us there).
 inline int kv_tile_query_rows(const KvAttnArgs& a, int max_rows) {
   const int64_t r = (int64_t)(max_rows ? std::min(max_rows, a.b.rows) : a.b.rows) * (a.heads / a.pool.nkv);
-  return r <= 8 ? 8 : r <= 16 ? 16 : r <= 32 ? 32 : r <= 64 || a.narrow ? 64 : 128;
+  if (!a.narrow && r > (a.chunk ? 64 : 32)) return 128;
+  return r <= 8 ? 8 : r <= 16 ? 16 : r <= 32 ? 32 : 64;
 }
 inline int64_t kv_tiles_bound(const KvAttnArgs& a, int tq) {
   const int64_t r = (int64_t)a.b.rows * (a.heads / a.pool.nkv);
@@ -162,34 +188,42 @@ inline int64_t kv_tiles_bound(const KvAttnArgs& a, int tq) {
   return r / tq + std::min(a.b.seqs, a.b.rows);
 }
 
-
-// Fills chunk (where it is 0) and slots; the workspace bytes.
+// Fills tq, chunk (where it is 0) and slots; the workspace bytes.
 inline size_t kv_plan(KvAttnArgs& a, int max_rows) {
   const int group = a.heads / a.pool.nkv, tq = kv_tile_query_rows(a, max_rows);
+  a.tq = tq;
   const int64_t cap = (int64_t)a.b.table_cols * a.pool.page_tokens;
   const int tile_tokens = (tq - 1) / group + 1;
   const int64_t span = a.window ? std::min<int64_t>(cap, (int64_t)a.window + a.sinks + tile_tokens + kKvTile) : cap;
-  const int64_t items = kv_tiles_bound(a, tq) * a.pool.nkv;
-  if (!a.chunk && tq <= 64) {
-    // Halve the split until two CTAs an SM have two chunks each to take, or a
-    // chunk is two tiles.
-    int64_t chunk = std::max<int64_t>(align_up(span, kKvTile), 2 * kKvTile);
-    while (chunk > 2 * kKvTile && items * ceil_div(span, chunk) < 4 * 148) chunk = align_up(chunk / 2, kKvTile);
-    a.chunk = (int)chunk;
-  } else if (!a.chunk) {
-    // One CTA an SM: the split n with the least waves x (tiles of a CTA + what
-    // a CTA costs besides) + the join of n partial results, in tiles' time
-    // (hd / 256 of about 0.7 us, twice that for f32 rows; a CTA's start and
-    // end cost some 6 us, partial results cross HBM twice).
-    const double tile_us = 0.7 * a.pool.hd / 256 * (a.dtype == F32 ? 2 : 1) + 0.4;
-    const double result_us = (double)a.b.rows * a.heads * a.pool.hd * 8 / 5e6;
+  if (!a.chunk) {
+    // The split n with the least estimated time, in us: CTAs run in waves of
+    // `ctas` an SM; a wave costs its tiles, at the SM's share of what bounds
+    // them, and a start and an end that nothing hides; n > 1 adds partial
+    // results that cross HBM twice and the join.  Tiles: the cache's bytes at
+    // 44 KB a us and SM; in the split kernel at least 0.4 us for 8 rows (twice
+    // that for f32 rows) at hd 256, in the tensor-core kernel 1.1 us (1.8).
+    const bool wide = tq == 128, f32 = a.dtype == F32;
+    const int elt = a.pool.format == kKvI8 ? 1 : 2;
+    const double read = (2.0 * kKvTile * a.pool.hd * elt + 512) / 43.9e3;
+    const double work = (wide ? 0.7 * (f32 ? 2 : 1) * a.pool.hd / 256 + 0.4
+                              : 0.4 * (tq / 8) * (f32 ? 2 : 1) * a.pool.hd / 256);
+    const double tile = std::max(read, work), fixed = 6;
+    const int64_t sms = 148, ctas = wide ? 1 : kv_narrow(a.pool.format, a.pool.hd, tq / 8, f32).ctas;
+    // (the tiles there will be, as far as max_rows tells, not the most possible)
+    const int64_t rows = max_rows ? std::min(max_rows, a.b.rows) : a.b.rows;
+    const int64_t items = std::min(kv_tiles_bound(a, tq), a.b.seqs * ceil_div(rows * group, tq)) * a.pool.nkv;
+    const double result = (double)a.b.rows * a.heads * a.pool.hd * 8 / 5e6;
+    const int64_t most = std::min<int64_t>(wide ? 64 : 512, std::max<int64_t>(span / (2 * kKvTile), 1));
     double best = 0;
-    for (int n = 1; n <= 16; n++) {
+    for (int64_t n = 1; n <= most; n += 1 + n / 16) {
       // (unsplit, a chunk holds all of the table: first tokens and window in one)
       const int64_t chunk = align_up(n == 1 ? std::max<int64_t>(cap, 1) : ceil_div(span, n), kKvTile);
-      const int64_t slots = n == 1 ? 1 : ceil_div(span, chunk) + (a.window ? 1 + (a.sinks > 0) : 0);
-      const double cost = (double)ceil_div(items * slots, 148) * (ceil_div(ceil_div(span, n), kKvTile) * tile_us + 6) +
-                          (n > 1 ? slots * result_us + 4 : 0);
+      const int64_t slots = n == 1 ? 1 : ceil_div(span, chunk) + (a.window && a.sinks ? 1 : 0);
+      const int64_t all = items * slots, full = all / (sms * ctas), rest = all % (sms * ctas);
+      const double tiles = (double)ceil_div(ceil_div(span, n), kKvTile);
+      double cost = full * (tiles * tile * ctas + fixed);
+      if (rest) cost += tiles * std::max(tile * ceil_div(rest, sms), 1.0) + fixed;
+      if (n > 1) cost += 3 + slots * result;
       if (n == 1 || cost < best) best = cost, a.chunk = (int)chunk;
     }
   }

@@ -600,7 +600,7 @@ int state_kv_attention(iq_state* s, int fi, const int* pos, int rows, const floa
   IQ_CHECK(ws.bytes >= need, IQ_ESTATE, "attention workspace of %zu bytes, %zu are needed", ws.bytes, need);
   kv_attend_bind(a, ws.p);
   s->launch_count += a.slots > 1 ? 2 : 1;
-  IQ_CUDA(kv_attend_launch(a, rows, s->st));
+  IQ_CUDA(kv_attend_launch(a, s->st));
   return IQ_OK;
 }
 

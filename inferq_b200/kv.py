@@ -83,16 +83,21 @@ class KvBatch:
             raise ValueError(f"row_start has {row_start.shape[0]} entries for {seqs} sequences")
         if max_rows < 0:
             raise ValueError("max_rows cannot be negative")
-        self.device = table.device
+        self.device, self.index = table.device, table.get_device()
         self.seqs = seqs
         self._keep = table, position, row_start
         ld = table.stride(0) if seqs > 1 else max(table.stride(0), table.shape[1])
         self._c = _Batch(table.data_ptr(), position.data_ptr(), None if row_start is None else row_start.data_ptr(), ld,
                          table.shape[1], seqs, 0, max_rows)
+        self._of_rows: dict[int, _Batch] = {}
 
     def _with(self, rows: int) -> _Batch:
-        c = self._c
-        return _Batch(c.table, c.position, c.row_start, c.table_ld, c.table_cols, c.seqs, rows, c.max_rows)
+        got = self._of_rows.get(rows)
+        if got is None:
+            c = self._c
+            got = _Batch(c.table, c.position, c.row_start, c.table_ld, c.table_cols, c.seqs, rows, c.max_rows)
+            self._of_rows[rows] = got
+        return got
 
 
 class KvCache:
@@ -111,6 +116,8 @@ class KvCache:
             _lib.check(self._lib.iq_kv_create(FORMATS[format], kv_heads, head_dim, page_tokens, pages, ctypes.byref(h)))
             self.device = torch.device("cuda", torch.cuda.current_device())
         self._h = h
+        self._index = self.device.index
+        self._attn: dict[tuple, _Attn] = {}
 
     @property
     def nbytes(self) -> int:
@@ -119,18 +126,21 @@ class KvCache:
         return n.value
 
     def _stream(self, stream):
-        return torch.cuda.current_stream(self.device).cuda_stream if stream is None else stream
+        # (the handle alone: current_stream() builds a stream object, 2 us a call)
+        return torch._C._cuda_getCurrentRawStream(self._index) if stream is None else stream
 
     def _rows(self, name, x, heads, batch):
+        shape = x.shape
         if x.dtype not in _TYPES:
             raise ValueError(f"{name} must be float32, float16 or bfloat16, got {x.dtype}")
-        if x.device != self.device or batch.device != self.device:
+        if x.get_device() != self._index or batch.index != self._index:
             raise ValueError(f"{name} and the batch must be on the cache's device {self.device}")
-        if x.dim() != 3 or x.shape[2] != self.head_dim or (heads and x.shape[1] != heads):
-            raise ValueError(f"{name} must be [rows, {heads or 'heads'}, {self.head_dim}], got {list(x.shape)}")
-        if x.stride(2) != 1:
+        if len(shape) != 3 or shape[2] != self.head_dim or (heads and shape[1] != heads):
+            raise ValueError(f"{name} must be [rows, {heads or 'heads'}, {self.head_dim}], got {list(shape)}")
+        row, head, elt = x.stride()
+        if elt != 1:
             raise ValueError(f"the elements of a head of {name} must be contiguous")
-        return x.data_ptr(), x.stride(0), x.stride(1)
+        return x.data_ptr(), row, head
 
     def append(self, k: torch.Tensor, v: torch.Tensor, batch: KvBatch, *, stream=None) -> None:
         """Quantise rows [rows, kv_heads, head_dim] into the cache."""
@@ -157,24 +167,27 @@ class KvCache:
         """Causal attention of rows ``q`` [rows, heads, head_dim] over their
         sequences' cached tokens (which include the rows' own: append first);
         see iq_kv_attend for ``window``, ``sinks``, ``scale`` and ``chunk``."""
-        rows, heads = q.shape[0], q.shape[1] if q.dim() == 3 else 0
         a = self._rows("queries", q, 0, batch)
+        rows, heads, _ = q.shape
         if out is None:
-            out = torch.empty(rows, heads, self.head_dim, dtype=q.dtype, device=self.device)
+            out = torch.empty((rows, heads, self.head_dim), dtype=q.dtype, device=q.device)
         elif out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError("queries and outputs must have one shape and type")
         b = self._rows("outputs", out, heads, batch)
-        c, at = batch._with(rows), _Attn(_TYPES[q.dtype], heads, scale, window, sinks, chunk)
-        need = ctypes.c_size_t()
-        _lib.check(self._lib.iq_kv_attend_workspace(self._h, c, at, ctypes.byref(need)))
-        ws = None
-        if need.value:
+        key = q.dtype, heads, scale, window, sinks, chunk
+        at = self._attn.get(key)
+        if at is None:
+            at = self._attn[key] = _Attn(_TYPES[q.dtype], heads, scale, window, sinks, chunk)
+        c, need = batch._with(rows), ctypes.c_size_t()
+        _lib.check(self._lib.iq_kv_attend_workspace(self._h, c, at, need))
+        ws, n = None, need.value
+        if n:
             if stream is None:
-                ws = torch.empty(need.value, dtype=torch.uint8, device=self.device)
+                ws = torch.empty(n, dtype=torch.uint8, device=q.device)
             else:  # the workspace belongs to the stream that uses it
                 with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=self.device)):
-                    ws = torch.empty(need.value, dtype=torch.uint8, device=self.device)
-        _lib.check(self._lib.iq_kv_attend(self._h, c, at, *a, *b, None if ws is None else ws.data_ptr(), need.value,
+                    ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+        _lib.check(self._lib.iq_kv_attend(self._h, c, at, *a, *b, None if ws is None else ws.data_ptr(), n,
                                           self._stream(stream)))
         return out
 
@@ -185,7 +198,7 @@ class KvCache:
 
     def __del__(self):
         h = getattr(self, "_h", None)
-        if h is not None and _lib._lib is not None:
+        if h is not None and _lib is not None and _lib._lib is not None:
             torch.cuda.synchronize(self.device)
             _lib._lib.iq_kv_destroy(h)
             self._h = None

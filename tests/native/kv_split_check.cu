@@ -19,6 +19,7 @@ int main(int argc, char** argv) {
   a.heads = arg(1);
   a.pool.nkv = arg(2);
   a.pool.hd = 64;
+  a.pool.format = kKvI8;
   a.pool.page_tokens = arg(3);
   a.pool.page_shift = __builtin_ctz(arg(3));
   a.b.table_cols = arg(4);
@@ -29,7 +30,7 @@ int main(int argc, char** argv) {
   a.sinks = a.window ? arg(8) : 0;
   a.chunk = arg(9);
   const size_t need = kv_plan(a, arg(10));
-  const int group = a.heads / a.pool.nkv, tq = kv_tile_query_rows(a, arg(10));
+  const int group = a.heads / a.pool.nkv, tq = a.tq;
   const int64_t cap = (int64_t)a.b.table_cols * a.pool.page_tokens;
   if ((need == 0) != (a.slots == 1)) return printf("workspace %zu for %d slots\n", need, a.slots), 1;
   const int tiles = (int)kv_tiles_bound(a, tq);

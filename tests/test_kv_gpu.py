@@ -483,3 +483,22 @@ def test_refusals(cuda):
     for scale in (0.3, -0.1):
         want, most = s.want(scale=scale)
         close(s.cache.attend(q, b, scale=scale), want, most, s.dt)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_every_short_quotient_is_rounded_right(cuda, dtype):
+    """Codes of 16-bit rows come from f32 quotients alone near a border: every significand of bf16 (a fourth of f16's)
+    over every one of the maximum's, in the binades that reach a code."""
+    dt, bits = DT[dtype], 8 if dtype == "bf16" else 11
+    m = torch.arange(1 << (bits - 1), 1 << bits).double() / (1 << (bits - 1))
+    x = torch.cat([m[::1 if bits == 8 else 4] * 2.0 ** -e for e in range(1, 9)]).to(dt)
+    hd = 64
+    x = x[: len(x) // 63 * 63].view(-1, 63)
+    for top in m[::1 if bits == 8 else 37]:
+        rows = torch.cat([torch.full((len(x), 1), float(top)).to(dt), x], 1).view(-1, 1, hd)
+        n = rows.shape[0]
+        cache = KvCache(1, hd, -(-n // 64), format="i8")
+        b = KvBatch(torch.arange(-(-n // 64), dtype=torch.int32, device="cuda").view(1, -1), torch.zeros(1, dtype=torch.int32, device="cuda"))
+        cache.append(rows.cuda(), rows.cuda(), b)
+        k, _ = cache.read(b, rows=n)
+        assert torch.equal(k.cpu(), held(rows, "i8").float())
