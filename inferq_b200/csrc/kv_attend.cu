@@ -296,15 +296,18 @@ __global__ void __launch_bounds__(160) kv_attend_kernel(const __grid_constant__ 
         }
 #pragma unroll
         for (int n = 0; n < NT; n++) {
+          float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int part = 0; part < (F32Q ? 2 : 1); part++) {
+          for (int part = F32Q ? 1 : 0; part >= 0; part--) {  // the small parts first
             const uint32_t at = qa + (part * TQ + n * 8) * QLD + 128 * j;
             const uint4 q0 = lds128(at), q1 = lds128(at + 16);
-            mma16816(sa[n], ka[0][0], ka[0][1], ka[0][2], ka[0][3], q0.x, q0.y);
-            mma16816(sa[n], ka[1][0], ka[1][1], ka[1][2], ka[1][3], q0.z, q0.w);
-            mma16816(sa[n], ka[2][0], ka[2][1], ka[2][2], ka[2][3], q1.x, q1.y);
-            mma16816(sa[n], ka[3][0], ka[3][1], ka[3][2], ka[3][3], q1.z, q1.w);
+            mma16816(x, ka[0][0], ka[0][1], ka[0][2], ka[0][3], q0.x, q0.y);
+            mma16816(x, ka[1][0], ka[1][1], ka[1][2], ka[1][3], q0.z, q0.w);
+            mma16816(x, ka[2][0], ka[2][1], ka[2][2], ka[2][3], q1.x, q1.y);
+            mma16816(x, ka[3][0], ka[3][1], ka[3][2], ka[3][3], q1.z, q1.w);
           }
+#pragma unroll
+          for (int c = 0; c < 4; c++) sa[n][c] += x[c];
         }
       }
       // ------------------------------------- scores, masks, tile maxima
@@ -349,7 +352,6 @@ __global__ void __launch_bounds__(160) kv_attend_kernel(const __grid_constant__ 
     ev = evn;
     const float v0 = sc[64 + 16 * warp + g] * up, v1 = sc[64 + 16 * warp + g + 8] * up;
     float fo[NT][2];
-    bool moved = false;
 #pragma unroll
     for (int n = 0; n < NT; n++) {
       float w[4];
@@ -363,7 +365,6 @@ __global__ void __launch_bounds__(160) kv_attend_kernel(const __grid_constant__ 
         const float p0 = ex2(sa[n][e] - ms), p1 = ex2(sa[n][2 + e] - ms);
         l[n][e] = l[n][e] * alpha + (p0 + p1);
         fo[n][e] = alpha * shrink;
-        moved |= fo[n][e] != 1.f;
         // a hidden token weighs zero whatever its scale is
         w[e] = sa[n][e] == -INFINITY ? 0.f : p0 * v0;
         w[2 + e] = sa[n][2 + e] == -INFINITY ? 0.f : p1 * v1;
@@ -379,25 +380,19 @@ __global__ void __launch_bounds__(160) kv_attend_kernel(const __grid_constant__ 
     consumers_sync();
     // --------------------------------------------------- O^T += V^T P^T
     if (sums) {
-      if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-        for (int b = 0; b < kMine; b++)
+      for (int b = 0; b < kMine; b++) {
+        const int blk = warp * kMine + b;
+        float x[2][NT][4];
 #pragma unroll
-          for (int m = 0; m < 2; m++)
+        for (int m = 0; m < 2; m++)
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
-              o[b][m][n][0] *= fo[n][0];
-              o[b][m][n][1] *= fo[n][1];
-              o[b][m][n][2] *= fo[n][0];
-              o[b][m][n][3] *= fo[n][1];
-            }
-      }
+          for (int n = 0; n < NT; n++)
 #pragma unroll
-      for (int kk = 0; kk < 4; kk++) {
-        uint32_t va[kMine][2][4];
+            for (int c = 0; c < 4; c++) x[m][n][c] = 0.f;
 #pragma unroll
-        for (int b = 0; b < kMine; b++) {
-          const int blk = warp * kMine + b;
+        for (int kk = 0; kk < 4; kk++) {
+          uint32_t va[2][4];
           if constexpr (FMT == kKvI8) {
             uint32_t w[4];
 #pragma unroll
@@ -410,28 +405,34 @@ __global__ void __launch_bounds__(160) kv_attend_kernel(const __grid_constant__ 
                         x1 = biased4_to_f16(__byte_perm(w[0], w[1], 0x7362)),
                         y0 = biased4_to_f16(__byte_perm(w[2], w[3], 0x5140)),
                         y1 = biased4_to_f16(__byte_perm(w[2], w[3], 0x7362));
-            va[b][0][0] = x0.x, va[b][0][1] = x0.y, va[b][0][2] = y0.x, va[b][0][3] = y0.y;
-            va[b][1][0] = x1.x, va[b][1][1] = x1.y, va[b][1][2] = y1.x, va[b][1][3] = y1.y;
+            va[0][0] = x0.x, va[0][1] = x0.y, va[0][2] = y0.x, va[0][3] = y0.y;
+            va[1][0] = x1.x, va[1][1] = x1.y, va[1][2] = y1.x, va[1][3] = y1.y;
           } else {
             const int m = lane >> 3, tok = 16 * kk + (lane & 7) + (m >> 1) * 8;
 #pragma unroll
             for (int mt = 0; mt < 2; mt++) {
               const int c = blk * 4 + mt * 2 + (m & 1);
-              ldsm4t(va[b][mt], vt + ((c >> 3) * kTile + tok) * 128 + (((c & 7) ^ (tok & 7)) << 4));
+              ldsm4t(va[mt], vt + ((c >> 3) * kTile + tok) * 128 + (((c & 7) ^ (tok & 7)) << 4));
             }
           }
+#pragma unroll
+          for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int part = F32Q ? 1 : 0; part >= 0; part--) {
+              const uint2 w = ps[((part * NT + n) * 4 + kk) * 32 + lane];
+#pragma unroll
+              for (int mt = 0; mt < 2; mt++) mma16816(x[mt][n], va[mt][0], va[mt][1], va[mt][2], va[mt][3], w.x, w.y);
+            }
         }
+        // The tensor cores cut a sum off (2^-25 of it a step on average, always
+        // towards zero); a tile's sums are added to the rest by rounding
+        // additions, so that no cut accumulates over the tokens.
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+        for (int m = 0; m < 2; m++)
 #pragma unroll
-          for (int part = 0; part < (F32Q ? 2 : 1); part++) {
-            const uint2 w = ps[((part * NT + n) * 4 + kk) * 32 + lane];
+          for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int b = 0; b < kMine; b++)
-#pragma unroll
-              for (int mt = 0; mt < 2; mt++)
-                mma16816(o[b][mt][n], va[b][mt][0], va[b][mt][1], va[b][mt][2], va[b][mt][3], w.x, w.y);
-          }
+            for (int c = 0; c < 4; c++) o[b][m][n][c] = fmaf(o[b][m][n][c], fo[n][c & 1], x[m][n][c]);
       }
     }
     __syncwarp();

@@ -172,13 +172,14 @@ constexpr KvNarrow kv_narrow(int format, int hd, int nt, bool f32) {
 
 // Query rows of a tile: the fewest of 8, 16, 32, 64 that take a sequence's
 // rows of one KV head at once, or the tensor-core kernel's 128: above 64 rows
-// unless the call keeps to the other, and above 32 where the split is free
+// unless the call keeps to the other, and above 16 where the split is free
 // too (16 sequences over 4127 tokens, 8 heads to a KV head, f32 and bf16 rows:
-// of 4 rows 59 and 45 us here, 61 and 51 us there; of 8 rows 136 and 113 us
-// here, 65 and 54 us there).
+// of 2 rows 34 and 29 us with tiles of 16; of 4 rows 78 and 51 us with tiles of
+// 32; of 8 rows 159 and 124 us with tiles of 64; with tiles of 128 55 and 47 us
+// whichever of these).
 inline int kv_tile_query_rows(const KvAttnArgs& a, int max_rows) {
   const int64_t r = (int64_t)(max_rows ? std::min(max_rows, a.b.rows) : a.b.rows) * (a.heads / a.pool.nkv);
-  if (!a.narrow && r > (a.chunk ? 64 : 32)) return 128;
+  if (!a.narrow && r > (a.chunk ? 64 : 16)) return 128;
   return r <= 8 ? 8 : r <= 16 ? 16 : r <= 32 ? 32 : 64;
 }
 inline int64_t kv_tiles_bound(const KvAttnArgs& a, int tq) {
@@ -187,6 +188,12 @@ inline int64_t kv_tiles_bound(const KvAttnArgs& a, int tq) {
   if ((a.heads / a.pool.nkv) % tq == 0) return r / tq;
   return r / tq + std::min(a.b.seqs, a.b.rows);
 }
+
+// The most tokens that one accumulator of the tensor-core kernel sums, for the
+// cuts that its steps make (kv_attend_wide.cu).  f32 rows: relative error
+// 1.0e-6 over 640 tokens, 3.0e-6 over 2560, 9.4e-6 over 8192 (32-bit torch
+// operations: 1.4e-6); 16-bit rows' own rounding covers 32768 tokens' cuts.
+constexpr int kWideChunkF32 = 1536, kWideChunk = 32768;
 
 // Fills tq, chunk (where it is 0) and slots; the workspace bytes.
 inline size_t kv_plan(KvAttnArgs& a, int max_rows) {
@@ -202,31 +209,42 @@ inline size_t kv_plan(KvAttnArgs& a, int max_rows) {
     // results that cross HBM twice and the join.  Tiles: the cache's bytes at
     // 44 KB a us and SM; in the split kernel at least 0.4 us for 8 rows (twice
     // that for f32 rows) at hd 256, in the tensor-core kernel 1.1 us (1.8).
+    // Several sequences are taken to be of mixed lengths, two thirds of the
+    // table on average: an SM that got long ones only sets the time (64
+    // sequences of up to 8209 tokens: chunks of 2752, one wave of 384 CTAs, 94
+    // us, of 1536 72 us, of 768 80 us, of 256 96 us).
     const bool wide = tq == 128, f32 = a.dtype == F32;
     const int elt = a.pool.format == kKvI8 ? 1 : 2;
     const double read = (2.0 * kKvTile * a.pool.hd * elt + 512) / 43.9e3;
     const double work = (wide ? 0.7 * (f32 ? 2 : 1) * a.pool.hd / 256 + 0.4
                               : 0.4 * (tq / 8) * (f32 ? 2 : 1) * a.pool.hd / 256);
-    const double tile = std::max(read, work), fixed = 6;
+    const double tile = std::max(read, work), fixed = wide ? 14 : 6;
     const int64_t sms = 148, ctas = wide ? 1 : kv_narrow(a.pool.format, a.pool.hd, tq / 8, f32).ctas;
     // (the tiles there will be, as far as max_rows tells, not the most possible)
     const int64_t rows = max_rows ? std::min(max_rows, a.b.rows) : a.b.rows;
     const int64_t items = std::min(kv_tiles_bound(a, tq), a.b.seqs * ceil_div(rows * group, tq)) * a.pool.nkv;
     const double result = (double)a.b.rows * a.heads * a.pool.hd * 8 / 5e6;
-    const int64_t most = std::min<int64_t>(wide ? 64 : 512, std::max<int64_t>(span / (2 * kKvTile), 1));
+    const int64_t most = std::min<int64_t>(512, std::max<int64_t>(span / (2 * kKvTile), 1));
     double best = 0;
     for (int64_t n = 1; n <= most; n += 1 + n / 16) {
       // (unsplit, a chunk holds all of the table: first tokens and window in one)
       const int64_t chunk = align_up(n == 1 ? std::max<int64_t>(cap, 1) : ceil_div(span, n), kKvTile);
+      if (wide && chunk > (f32 ? kWideChunkF32 : kWideChunk) && n < most) continue;
       const int64_t slots = n == 1 ? 1 : ceil_div(span, chunk) + (a.window && a.sinks ? 1 : 0);
       const int64_t all = items * slots, full = all / (sms * ctas), rest = all % (sms * ctas);
       const double tiles = (double)ceil_div(ceil_div(span, n), kKvTile);
-      double cost = full * (tiles * tile * ctas + fixed);
-      if (rest) cost += tiles * std::max(tile * ceil_div(rest, sms), 1.0) + fixed;
+      double cost;
+      if (a.b.seqs > 1) {
+        cost = std::max(1.0, 0.65 * all / (sms * ctas)) * (tiles * tile * ctas + fixed);
+      } else {
+        cost = full * (tiles * tile * ctas + fixed);
+        if (rest) cost += tiles * std::max(tile * ceil_div(rest, sms), 1.0) + fixed;
+      }
       if (n > 1) cost += 3 + slots * result;
-      if (n == 1 || cost < best) best = cost, a.chunk = (int)chunk;
+      if (!a.chunk || cost < best) best = cost, a.chunk = (int)chunk;
     }
   }
+  if (tq == 128) a.chunk = std::min(a.chunk, a.dtype == F32 ? kWideChunkF32 : kWideChunk);
   const int64_t all = std::max<int64_t>(ceil_div(cap, a.chunk), 1);
   a.slots = (int)all;
   if (a.window)
