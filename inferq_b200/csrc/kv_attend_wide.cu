@@ -76,7 +76,7 @@ struct Geo {
   static constexpr uint32_t kTmemS = HD, kTmemQ = HD + 2 * kT;
   static constexpr uint32_t kTmemCols = HD + 2 * kT + HD / 2 > 256 ? 512 : 256;
   static_assert(HD + 2 * kT + HD / 2 <= 512, "O, S and Q fit the tensor memory");
-  static_assert((FMT == kKvI8 ? kRing : kRingV) * kTileBytes >= kM * HD * 2, "Q is staged where tiles come later");
+  static_assert(kRingV * kTileBytes >= kM * HD * 2 || (FMT == kKvI8 && kRing * kTileBytes >= kM * HD * 2), "Q is staged where tiles come later");
   static_assert(kStages >= (kStageTokens == kT ? 2 : 3) || FMT != kKvI8, "see the loader's turns");
   static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
 };
@@ -216,9 +216,10 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
   uint8_t* kring = smem;
   uint8_t* vring = smem + R * TB;
   uint8_t* qlo = vring + RV * TB;
-  // Q's first parts pass through a ring before its tiles come: f16 tiles of
-  // values are needed last, i8 tiles of keys are expanded behind their bytes
-  uint8_t* qring = FMT == kKvI8 ? kring : vring;
+  // Q's first parts pass through a ring before its tiles come: that of the
+  // values, which are needed last, where it is large enough
+  constexpr bool kQinV = RV * TB >= kM * HD * 2;
+  uint8_t* qring = kQinV ? vring : kring;
   uint8_t* stages = qlo + G_::kQlo;                                 // [keys, values][stage]
   float* scales = reinterpret_cast<float*>(stages + 2 * NS * SB);  // [ring][keys 64, values 64, exponent, pad]
   float* tops = scales + kScaleRing * (2 * kT + 4);  // [half][row] maxima of a tile
@@ -232,11 +233,26 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
   const int slot = blockIdx.x % a.slots;
   const int kvh = blockIdx.x / a.slots % p.nkv;
   const int tile = blockIdx.x / a.slots / p.nkv;
-  KvTileRows tr;
-  if (!kv_tile_rows(a.b, tile, kM, group, lane, &tr)) return;
-  const KvSpan sp = kv_span(a, tr, kM, slot);
-  if (sp.outside && threadIdx.x == 0) atomicOr(p.flag, kKvBadPage);
-  if (sp.first >= sp.end && a.slots > 1) return;
+  // One warp finds the tile's rows and tokens (a few hundred instructions, which
+  // 27 warps would issue in turn).
+  __shared__ KvTileRows tr_s;
+  __shared__ KvSpan sp_s;
+  if (warp == 0) {
+    KvTileRows t = {};
+    KvSpan s = {};
+    const bool any = kv_tile_rows(a.b, tile, kM, group, lane, &t);
+    if (any) s = kv_span(a, t, kM, slot);
+    if (lane == 0) {
+      if (!any) t.seq = -1;
+      if (any && s.outside) atomicOr(p.flag, kKvBadPage);
+      tr_s = t;
+      sp_s = s;
+    }
+  }
+  __syncthreads();
+  const KvTileRows tr = tr_s;
+  const KvSpan sp = sp_s;
+  if (tr.seq < 0 || (sp.first >= sp.end && a.slots > 1)) return;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < R; s++) {
@@ -299,16 +315,22 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
     const int pair = grp * 4 + quarter, part = warp >> 2;
     {
       constexpr int N = HD / 32, U = 4;  // rows in flight
-#pragma unroll 1  // (straight-line code that runs once costs its instruction fetch)
+      // where the warp's eight rows begin, one to a lane: -1 behind the last
+      // (divisions once a lane, not once a row: sixteen warps share the issue)
+      int64_t begin = -1;
+      {
+        const int rr = tr.r0 + r0 + 8 * part + (lane & 7);
+        const int i = rr / group, h = kvh * group + rr - i * group;
+        if (rr < tr.nr) begin = (int64_t)(tr.row0 + i) * a.q.row + (int64_t)h * a.q.head;
+      }
+#pragma unroll 1
       for (int rb = 8 * part; rb < 8 * part + 8; rb += U) {
         float x[U][N];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-          const int rr = tr.r0 + r0 + rb + u;
-          const bool live = rr < tr.nr;
-          const int i = rr / group, h = kvh * group + rr % group;
-          const int64_t o = (int64_t)(tr.row0 + i) * a.q.row + (int64_t)h * a.q.head + lane * N;
-          if (live) {
+          const int64_t at = __shfl_sync(0xffffffffu, begin, (rb & 7) + u);
+          const int64_t o = at + lane * N;
+          if (at >= 0) {
             if constexpr (F32Q) load_n<float, N>(static_cast<const float*>(a.q.p) + o, vec, x[u]);
             else if (a.dtype == F16) load_n<__half, N>(static_cast<const __half*>(a.q.p) + o, vec, x[u]);
             else load_n<__nv_bfloat16, N>(static_cast<const __nv_bfloat16*>(a.q.p) + o, vec, x[u]);
@@ -571,7 +593,7 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
             asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(base + at), "r"(su32(mine)),
                          "r"(HD * (int)sizeof(T))
                          : "memory");
-          asm volatile("cp.async.bulk.commit_group;\ncp.async.bulk.wait_group 0;" ::: "memory");
+          asm volatile("cp.async.bulk.commit_group;\ncp.async.bulk.wait_group.read 0;" ::: "memory");
         } else {
           for (int i = 8 * part; i < 8 * part + 8; i++) {
             const int64_t to = __shfl_sync(0xffffffffu, at, i);
@@ -772,7 +794,7 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
     constexpr int kPer = kT / G_::kStageTokens, NP = G_::kStageTokens / TP;  // stages a tile, passes a stage
     const int ch = tid % C, tk = tid / C;
     bool ok = true;
-    if (!isv && sp.first < sp.end) ok = wait(&qfull, 0);  // the K ring holds the query rows first
+    if (isv == kQinV && sp.first < sp.end) ok = wait(&qfull, 0);  // the ring holds the query rows first
     int it = 0;
     for (int ti = sp.first; ok && ti < sp.end; ti = sp.next(ti), it++) {
       const int s = it % rn;
