@@ -499,7 +499,7 @@ __global__ void __launch_bounds__(160) kv_attend_kernel(const __grid_constant__ 
 // over the chunks c that the row sees.  Chunk c belongs to group c mod 8; a
 // group's chunks are summed in order, then the groups in order, whichever
 // kernel does it: the result depends on the row's own chunks only.
-constexpr int kGroups = 8, kFewSlots = 32;
+constexpr int kGroups = 8;
 
 struct JoinRow {
   KvChunks ch;
@@ -526,16 +526,17 @@ __device__ __forceinline__ JoinRun join_run(const JoinRow& j, int r) {
   return {j.rc.window0, j.rc.window0 + j.rc.count - j.rc.firsts};
 }
 
-// One warp per (row, head), for many of those: the chunks in blocks of eight,
-// one to a group, all of a block's loads in flight at once.
+// Up to eight slots: one warp per (row, head).  A group has at most one chunk
+// of either list then, so groups are summed as they come, the loads of four of
+// them in flight.
 template <class T, int HD>
 __global__ void __launch_bounds__(128) kv_join_few_kernel(const __grid_constant__ KvAttnArgs a, const int tq,
                                                           const bool vec) {
   constexpr int N = HD / 32;
   pdl_wait();
   const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int row = (int)(item / a.heads), h = (int)(item % a.heads);
+  const uint32_t item = blockIdx.x * 4 + (threadIdx.x >> 5);  // (rows x heads below 2^31)
+  const int row = (int)(item / (uint32_t)a.heads), h = (int)(item - (uint32_t)row * a.heads);
   if (row >= a.b.rows) return;
   JoinRow j;
   if (!join_row(a, row, h, tq, lane, &j)) return;
@@ -544,43 +545,38 @@ __global__ void __launch_bounds__(128) kv_join_few_kernel(const __grid_constant_
   const float2 mine = lane < j.rc.count ? ml[j.ch.slot(j.rc.chunk(lane))] : make_float2(-INFINITY, 0.f);
   float M = mine.x;
 #pragma unroll
-  for (int w = 16; w; w >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, w));
+  for (int w = 4; w; w >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, w));
+  M = __shfl_sync(0xffffffffu, M, 0);
   const float wt = kvp::ex2(mine.x - (M == -INFINITY ? 0.f : M));
-  float acc[kGroups][N], sums[kGroups];
-#pragma unroll
-  for (int g = 0; g < kGroups; g++) {
-    sums[g] = 0.f;
-#pragma unroll
-    for (int k = 0; k < N; k++) acc[g][k] = 0.f;
-  }
-#pragma unroll 1
-  for (int r = 0; r < 2; r++) {
-    const JoinRun run = join_run(j, r);
-    const int at = (r ? j.rc.firsts : 0) - run.b;  // a chunk's place among the row's
-#pragma unroll 1
-    for (int c0 = run.b & ~(kGroups - 1); c0 < run.e; c0 += kGroups) {
-      float x[kGroups][N];
-#pragma unroll
-      for (int g = 0; g < kGroups; g++)
-        if (c0 + g >= run.b && c0 + g < run.e) load_n<float, N>(part + (int64_t)j.ch.slot(c0 + g) * HD, true, x[g]);
-#pragma unroll
-      for (int g = 0; g < kGroups; g++) {
-        const float w = __shfl_sync(0xffffffffu, wt, (c0 + g + at) & 31), l = __shfl_sync(0xffffffffu, mine.y, (c0 + g + at) & 31);
-        if (c0 + g < run.b || c0 + g >= run.e) continue;
-#pragma unroll
-        for (int k = 0; k < N; k++) acc[g][k] = fmaf(w, x[g][k], acc[g][k]);
-        sums[g] = fmaf(w, l, sums[g]);
-      }
-    }
-  }
   float o[N], sum = 0.f;
 #pragma unroll
   for (int k = 0; k < N; k++) o[k] = 0.f;
-#pragma unroll
+  const JoinRun first = join_run(j, 0), second = join_run(j, 1);
+  const int at = j.rc.firsts - second.b;  // a chunk's place among the row's
+#pragma unroll 4
   for (int g = 0; g < kGroups; g++) {
+    const int c0 = first.b + ((g - first.b) & (kGroups - 1)), c1 = second.b + ((g - second.b) & (kGroups - 1));
+    const bool in0 = c0 < first.e, in1 = c1 < second.e;
+    const float w0 = __shfl_sync(0xffffffffu, wt, c0 & 31), l0 = __shfl_sync(0xffffffffu, mine.y, c0 & 31);
+    const float w1 = __shfl_sync(0xffffffffu, wt, (c1 + at) & 31), l1 = __shfl_sync(0xffffffffu, mine.y, (c1 + at) & 31);
+    float t[N], x[N], s = 0.f;
 #pragma unroll
-    for (int k = 0; k < N; k++) o[k] += acc[g][k];
-    sum += sums[g];
+    for (int k = 0; k < N; k++) t[k] = 0.f;
+    if (in0) {
+      load_n<float, N>(part + (int64_t)j.ch.slot(c0) * HD, true, x);
+#pragma unroll
+      for (int k = 0; k < N; k++) t[k] = fmaf(w0, x[k], t[k]);
+      s = fmaf(w0, l0, s);
+    }
+    if (in1) {
+      load_n<float, N>(part + (int64_t)j.ch.slot(c1) * HD, true, x);
+#pragma unroll
+      for (int k = 0; k < N; k++) t[k] = fmaf(w1, x[k], t[k]);
+      s = fmaf(w1, l1, s);
+    }
+#pragma unroll
+    for (int k = 0; k < N; k++) o[k] += t[k];
+    sum += s;
   }
   const float f = sum != 0.f ? __fdiv_rn(1.f, sum) : 0.f;
 #pragma unroll
@@ -696,9 +692,7 @@ template <class T, int HD>
 cudaError_t launch_join(const KvAttnArgs& a, int tq, cudaStream_t st) {
   const int64_t items = (int64_t)a.b.rows * a.heads;
   const bool vec = strides_ok(a.out, sizeof(T), 16);
-  // a warp each where there are warps enough for the GPU (8 an SM), or little
-  // to join
-  if (a.slots <= kFewSlots && (items >= 8 * 148 || a.slots <= kGroups))
+  if (a.slots <= kGroups)
     return launch_pdl(kv_join_few_kernel<T, HD>, dim3((unsigned)ceil_div(items, 4)), dim3(128), 0, st, true, a, tq, vec);
   return launch_pdl(kv_join_kernel<T, HD>, dim3((unsigned)items), dim3(256), 0, st, true, a, tq, vec);
 }
