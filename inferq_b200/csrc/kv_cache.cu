@@ -52,39 +52,50 @@ __device__ __noinline__ float code_f64(float x, float amax) {
 }
 
 // Biased codes of N elements; amax finite and above zero.  kShort: x and amax
-// have at most 11 significant bits (f16 and bf16 rows).  A quotient 127 x /
-// amax that is no tie then lies at least 2^-20 of itself from one ((254 mx 2^k
-// - (2n + 1) ma) / 2 ma is a multiple of 2^k / 2 ma with ma < 2^11 and 2^k >=
-// q / 254), and the f32 product is within 2^-23: what lies within 2^-21 of a
-// border is a tie, and goes to the even side.  16-bit rows meet ties in up to
-// 40% of their vectors.
+// have at most 11 significant bits (f16 and bf16 rows, up to 40% of whose
+// vectors meet a tie).  127 x is exact then, and a quotient that is no tie lies
+// at least 2^-20 of itself from one ((254 mx 2^k - (2n + 1) ma) / 2 ma is a
+// multiple of 2^k / 2 ma with ma < 2^11 and 2^k >= q / 254): a quotient
+// corrected by its exact remainder is a tie where the real one is, and on the
+// right side otherwise.
 template <int N, bool kShort>
 __device__ __forceinline__ void codes_i8(const float (&x)[N], float amax, uint8_t* out) {
-  float far = 0.f, t[N], d[N];
-  const bool middle = amax > 0x1p-100f && amax < 0x1p100f;  // else the factor or a product leaves f32's normals
-  const float c = middle ? __fdiv_rn(127.f, amax) : 0.f;
-#pragma unroll
-  for (int j = 0; j < N; j += 2) {
-    const float2 v = kvp::mul2(make_float2(x[j], x[j + 1]), make_float2(c, c));
-    const float2 u = kvp::add2(v, make_float2(kMagic, kMagic));
-    const float2 r = kvp::add2(u, make_float2(-kMagic, -kMagic));
-    const float2 e = kvp::add2(v, make_float2(-r.x, -r.y));
-    t[j] = u.x;
-    t[j + 1] = u.y;
-    d[j] = e.x;
-    d[j + 1] = e.y;
-    far = fmaxf(far, fmaxf(fabsf(e.x), fabsf(e.y)));
-  }
-  constexpr float kNear = 0.5f - 0x1p-15f;
-  if (far > kNear || !middle) {
+  float t[N];
+  if (!(amax > 0x1p-100f && amax < 0x1p100f)) {  // a factor or a product would leave f32's normals
 #pragma unroll  // (an index that varies would put the arrays in local memory)
-    for (int j = 0; j < N; j++) {
-      if (kShort && middle) {
-        const bool tie = 0.5f - fabsf(d[j]) < fabsf(x[j] * c) * 0x1p-21f;
-        if (tie && (__float_as_uint(t[j]) & 1)) t[j] += copysignf(1.f, d[j]);
-      } else if (fabsf(d[j]) > kNear || !middle) {
-        t[j] = code_f64(x[j], amax);
-      }
+    for (int j = 0; j < N; j++) t[j] = code_f64(x[j], amax);
+  } else if constexpr (kShort) {
+    const float inv = __fdiv_rn(1.f, amax);
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+      const float2 num = kvp::mul2(make_float2(x[j], x[j + 1]), make_float2(127.f, 127.f));
+      float2 q = kvp::mul2(num, make_float2(inv, inv));
+      const float2 left = kvp::fma2(make_float2(-q.x, -q.y), make_float2(amax, amax), num);
+      q = kvp::fma2(left, make_float2(inv, inv), q);
+      q = kvp::add2(q, make_float2(kMagic, kMagic));
+      t[j] = q.x;
+      t[j + 1] = q.y;
+    }
+  } else {
+    const float c = __fdiv_rn(127.f, amax);
+    float far = 0.f, d[N];
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+      const float2 v = kvp::mul2(make_float2(x[j], x[j + 1]), make_float2(c, c));
+      const float2 u = kvp::add2(v, make_float2(kMagic, kMagic));
+      const float2 r = kvp::add2(u, make_float2(-kMagic, -kMagic));
+      const float2 e = kvp::add2(v, make_float2(-r.x, -r.y));
+      t[j] = u.x;
+      t[j + 1] = u.y;
+      d[j] = fabsf(e.x);
+      d[j + 1] = fabsf(e.y);
+      far = fmaxf(far, fmaxf(d[j], d[j + 1]));
+    }
+    constexpr float kNear = 0.5f - 0x1p-15f;
+    if (far > kNear) {
+#pragma unroll
+      for (int j = 0; j < N; j++)
+        if (d[j] > kNear) t[j] = code_f64(x[j], amax);
     }
   }
   if constexpr (N == 2) {
@@ -196,7 +207,7 @@ __global__ void __launch_bounds__(256, 5) kv_append_kernel(const __grid_constant
 
 // The reverse; rows at negative positions or behind the table read as zeros.
 template <class T, int HD, int FMT>
-__global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ KvPool p, const __grid_constant__ KvBatch b,
+__global__ void __launch_bounds__(256, 6) kv_read_kernel(const __grid_constant__ KvPool p, const __grid_constant__ KvBatch b,
                                                       KvTensor k, KvTensor v, bool vec, int turns) {
   constexpr int N = HD / 32;
   constexpr int kB = FMT == kKvI8 ? N : 2 * N;
@@ -206,7 +217,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ Kv
   if (threadIdx.x < 8 * turns && item0 + threadIdx.x < items)
     places[threadIdx.x] = place_of(p, b, (int)((item0 + threadIdx.x) / (uint32_t)p.nkv));
   __syncthreads();
-#pragma unroll 2
+#pragma unroll 1  // (two turns unrolled: 71 us instead of 61 for 65536 f32 rows, by their registers)
   for (int turn = 0; turn < turns; turn++) {
     const uint32_t item = item0 + turn * 8 + warp;
     if (item >= items) return;
