@@ -107,14 +107,6 @@ __device__ __forceinline__ void codes_i8(const float (&x)[N], float amax, uint8_
   }
 }
 
-template <int B>
-__device__ __forceinline__ void copy_bytes(void* dst, const void* src) {
-  if constexpr (B == 16) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
-  else if constexpr (B == 8) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(src);
-  else if constexpr (B == 4) *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(src);
-  else *reinterpret_cast<uint16_t*>(dst) = *reinterpret_cast<const uint16_t*>(src);
-}
-
 // Where the CTA's items (row, KV head) lie, found by one thread each: a page
 // and a token in it, kNoRow behind the last sequence, kPadding at a negative
 // position, -1 outside the table or the pool.

@@ -110,6 +110,15 @@ __device__ __forceinline__ void store_n(T* p, bool vec, const float (&x)[N]) {
   }
 }
 
+// B bytes as one access.
+template <int B>
+__device__ __forceinline__ void copy_bytes(void* dst, const void* src) {
+  if constexpr (B == 16) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
+  else if constexpr (B == 8) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(src);
+  else if constexpr (B == 4) *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(src);
+  else *reinterpret_cast<uint16_t*>(dst) = *reinterpret_cast<const uint16_t*>(src);
+}
+
 // Exponent e of the power of two that brings a vector of largest magnitude
 // `amax` to [2^14, 2^15) as x / 2^e: inside f16's normal range with 28
 // binades below.  0 for a non-finite maximum; at least -126, so that 2^e and
