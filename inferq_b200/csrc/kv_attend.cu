@@ -112,7 +112,7 @@ struct Geo {
 };
 
 template <int HD, int FMT, int NT, bool F32Q>
-__global__ void __launch_bounds__(160) kv_attend_kernel(const __grid_constant__ KvAttnArgs a, const bool vec) {
+__global__ void __launch_bounds__(160, NT == 1 ? 3 : 1) kv_attend_kernel(const __grid_constant__ KvAttnArgs a, const bool vec) {
   using G_ = Geo<HD, FMT, NT, F32Q>;
   constexpr int TQ = G_::kTQ, ST = G_::kStages, QLD = G_::kQld;
   __shared__ __align__(8) uint64_t full[ST], empty[ST];

@@ -210,9 +210,10 @@ inline size_t kv_plan(KvAttnArgs& a, int max_rows) {
     // 44 KB a us and SM; in the split kernel at least 0.4 us for 8 rows (twice
     // that for f32 rows) at hd 256, in the tensor-core kernel 1.1 us (1.8).
     // Several sequences are taken to be of mixed lengths, two thirds of the
-    // table on average: an SM that got long ones only sets the time (64
-    // sequences of up to 8209 tokens: chunks of 2752, one wave of 384 CTAs, 94
-    // us, of 1536 72 us, of 768 80 us, of 256 96 us).
+    // table on average: an SM that got long ones only sets the time (64 bf16
+    // sequences of up to 8209 tokens, i8, hd 256: chunks of 8256 take 136 us,
+    // of 4160 94, of 2048 69, of 1024 78, of 256 91, of 128 116; the rule's
+    // 1408 takes 85, and 64 sequences of 6000 tokens 78 of at best 72).
     const bool wide = tq == 128, f32 = a.dtype == F32;
     const int elt = a.pool.format == kKvI8 ? 1 : 2;
     const double read = (2.0 * kKvTile * a.pool.hd * elt + 512) / 43.9e3;
