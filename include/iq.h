@@ -375,11 +375,13 @@ int iq_kv_bytes(const iq_kv* c, int64_t* bytes);
 
 /* Quantise rows [row][kv_head][head_dim] of keys and values (dtype IQ_F32,
  * IQ_F16 or IQ_BF16; strides in elements, elements of a head contiguous) into
- * the cache.  Rows of one call must have positions of their own. */
+ * the cache.  Rows of one call must have places of their own: no two rows at
+ * one position of a sequence, nor at one token of a page that sequences share. */
 int iq_kv_append(iq_kv* c, const iq_kv_batch* b, int dtype, const void* k, int64_t k_row, int64_t k_head,
                  const void* v, int64_t v_row, int64_t v_head, void* stream);
 /* The reverse: the values that the cache holds at the rows' positions, in
- * `dtype`; rows at negative positions are zeros. */
+ * `dtype`, keys and values to places of their own; rows at negative positions
+ * are zeros. */
 int iq_kv_read(const iq_kv* c, const iq_kv_batch* b, int dtype, void* k, int64_t k_row, int64_t k_head, void* v,
                int64_t v_row, int64_t v_head, void* stream);
 
@@ -392,11 +394,16 @@ int iq_kv_read(const iq_kv* c, const iq_kv_batch* b, int dtype, void* k, int64_t
  * are f32, f32 queries and weights enter the matrix instructions as two f16
  * parts each, others rounded to f16 (a row's queries over a power of two, so
  * that bf16's range is kept).
+ * out may be q itself (with its strides); no other overlap is allowed.
  * chunk: tokens per split of a sequence (a multiple of 64), counted from
  * position 0, whose partial results are joined in order; 0 lets the call
  * choose by the batch's bounds.  With a chunk given and at most 64 query rows
  * a sequence and KV head (max_rows * heads / kv_heads), a row's result
- * depends on its own context and chunk only, bit for bit. */
+ * depends on its own context and chunk only, bit for bit.  More query rows
+ * run on the tcgen05 tensor cores (from 17, where the call chooses the
+ * chunk), where a split is at most 1536 tokens for IQ_F32 and 32768
+ * otherwise: longer ones are cut to that, since the accumulators round
+ * towards zero. */
 typedef struct iq_kv_attn {
   int32_t dtype;
   int32_t heads;

@@ -7,6 +7,10 @@
 
 namespace iq {
 
+// An entry of row_start, within the batch's rows whatever the caller wrote:
+// counts and products of rows cannot overflow.
+__device__ __forceinline__ int kv_row(const KvBatch& b, int at) { return min(max(at, 0), b.rows); }
+
 // Sequence of `row` (warp-wide; every lane returns it), the row's index in it,
 // the sequence's rows and its first position; -1 when the row lies behind the
 // last sequence.  row_start ascends; each round narrows the range 32-fold, and
@@ -27,7 +31,7 @@ __device__ __forceinline__ KvSeq kv_seq_of_row(const KvBatch& b, int row, int la
     n = min(step, b.seqs - lo);
   }
   const int s = min(lo + lane, b.seqs - 1);
-  const int begin = b.row_start[s], end = b.row_start[s + 1], pos = b.position[s];
+  const int begin = kv_row(b, b.row_start[s]), end = kv_row(b, b.row_start[s + 1]), pos = b.position[s];
   const uint32_t past = __ballot_sync(0xffffffffu, lane < n && end > row);
   if (!past) return {-1, 0, 0, 0};
   const int at = __ffs(past) - 1;

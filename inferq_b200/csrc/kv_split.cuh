@@ -48,7 +48,7 @@ __device__ __forceinline__ bool kv_tile_rows(const KvBatch& b, int tile, int tq,
     t->seq = -1;
     for (int s0 = 0; s0 < b.seqs; s0 += 32) {
       const int s = min(s0 + lane, b.seqs - 1);
-      const int begin = b.row_start[s], end = b.row_start[s + 1], pos = b.position[s];
+      const int begin = kv_row(b, b.row_start[s]), end = kv_row(b, b.row_start[s + 1]), pos = b.position[s];
       const int rows = s0 + lane < b.seqs ? max(end - begin, 0) : 0;
       const int tiles = (int)(((int64_t)rows * group + tq - 1) / tq);
       int sum = tiles;
@@ -71,7 +71,7 @@ __device__ __forceinline__ bool kv_tile_rows(const KvBatch& b, int tile, int tq,
     }
     if (t->seq < 0) return false;
   }
-  if (t->row0 < 0) return false;
+  if (t->r0 < 0) return false;  // (a row_start so wrong that the tiles' number overflows)
   t->nr = min(n, b.rows - t->row0) * group;
   return t->r0 < t->nr;
 }
@@ -86,7 +86,7 @@ struct KvChunks {
 __host__ __device__ inline KvChunks kv_chunks(const KvAttnArgs& a, int64_t pa) {
   KvChunks c = {0, 0};
   if (a.window) {
-    c.first_chunks = (a.sinks + a.chunk - 1) / a.chunk;
+    c.first_chunks = a.sinks ? (a.sinks - 1) / a.chunk + 1 : 0;  // (no sum that passes 31 bits)
     c.window0 = (int)kv_max(c.first_chunks, kv_clip(pa - a.window + 1) / a.chunk);
   }
   return c;
@@ -136,8 +136,8 @@ __host__ __device__ inline KvSpan kv_span(const KvAttnArgs& a, const KvTileRows&
   const int64_t pa = t.pos + t.r0 / group, pb = t.pos + ((int)kv_min(t.r0 + tq, t.nr) - 1) / group;
   const int64_t top = (1ll << 31) - 1;
   KvSpan s;
-  s.pa = (int)kv_max(kv_min(pa, top), -top);
-  s.pb = (int)kv_max(kv_min(pb, top), -top);
+  s.pa = (int)kv_max(kv_min(pa, top), -1);  // (any negative position is padding; less a window it stays in 32 bits)
+  s.pb = (int)kv_max(kv_min(pb, top), -1);
   s.outside = pb >= cap;
   s.tokens = (int)kv_max(kv_min(pb + 1, cap), 0);
   s.window = a.window;
@@ -200,6 +200,11 @@ inline size_t kv_plan(KvAttnArgs& a, int max_rows) {
   const int group = a.heads / a.pool.nkv, tq = kv_tile_query_rows(a, max_rows);
   a.tq = tq;
   const int64_t cap = (int64_t)a.b.table_cols * a.pool.page_tokens;
+  // what reaches past the table says no more than the table's end
+  const int end = (int)align_up(cap + 1, kKvTile);
+  a.window = std::min(a.window, end);
+  a.sinks = std::min(a.sinks, end);
+  a.chunk = std::min(a.chunk, end);
   const int tile_tokens = (tq - 1) / group + 1;
   const int64_t span = a.window ? std::min<int64_t>(cap, (int64_t)a.window + a.sinks + tile_tokens + kKvTile) : cap;
   if (!a.chunk) {

@@ -129,6 +129,16 @@ class KvCache:
         # (the handle alone: current_stream() builds a stream object, 2 us a call)
         return torch._C._cuda_getCurrentRawStream(self._index) if stream is None else stream
 
+    def _new(self, shape, dtype, stream):
+        """Memory of the stream that writes it; the current one may read it."""
+        if stream is None:
+            return torch.empty(shape, dtype=dtype, device=self.device)
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=self.device)):
+            x = torch.empty(shape, dtype=dtype, device=self.device)
+        if x.numel():
+            x.record_stream(torch.cuda.current_stream(self.device))
+        return x
+
     def _rows(self, name, x, heads, batch):
         shape = x.shape
         if x.dtype not in _TYPES:
@@ -154,7 +164,7 @@ class KvCache:
         rows behind the last sequence are left as they are in ``out``."""
         if out is None:
             shape = (rows, self.kv_heads, self.head_dim)
-            out = tuple(torch.empty(shape, dtype=dtype, device=self.device) for _ in range(2))
+            out = self._new(shape, dtype, stream), self._new(shape, dtype, stream)
         k, v = out
         if k.shape != v.shape or k.dtype != v.dtype or k.shape[0] != rows:
             raise ValueError("keys and values must have one shape and type, and the batch's rows")
@@ -170,7 +180,7 @@ class KvCache:
         a = self._rows("queries", q, 0, batch)
         rows, heads, _ = q.shape
         if out is None:
-            out = torch.empty((rows, heads, self.head_dim), dtype=q.dtype, device=q.device)
+            out = self._new((rows, heads, self.head_dim), q.dtype, stream)
         elif out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError("queries and outputs must have one shape and type")
         b = self._rows("outputs", out, heads, batch)
@@ -182,11 +192,7 @@ class KvCache:
         _lib.check(self._lib.iq_kv_attend_workspace(self._h, c, at, need))
         ws, n = None, need.value
         if n:
-            if stream is None:
-                ws = torch.empty(n, dtype=torch.uint8, device=q.device)
-            else:  # the workspace belongs to the stream that uses it
-                with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=self.device)):
-                    ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+            ws = self._new(n, torch.uint8, stream)
         _lib.check(self._lib.iq_kv_attend(self._h, c, at, *a, *b, None if ws is None else ws.data_ptr(), n,
                                           self._stream(stream)))
         return out

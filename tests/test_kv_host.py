@@ -92,6 +92,10 @@ def _split_cases():
         (16, 2, 64, 4, 5, -9, 7, 2, 64, 5), (16, 2, 64, 2, 9, 125, 0, 0, 64, 9), (4, 4, 128, 8, 70, 900, 64, 64, 128, 1),
         (16, 2, 64, 0, 2, 0, 0, 0, 64, 2), (128, 1, 16, 40, 4, 600, 100, 130, 64, 4),
     ]
+    most = 2**31 - 1  # the types' ends
+    cases += [(16, 2, 64, 9, rows, p, window, sinks, chunk, max_rows) for rows, p in ((1, 300), (5, -2), (70, 300))
+              for window, sinks in ((most, 0), (most, most), (1, most), (most, 70)) for chunk in (0, 64, most - 63)
+              for max_rows in (0, most)]
     for _ in range(150):
         kv_heads = int(r.choice([1, 2, 3]))
         page, cols, rows = int(r.choice([16, 32, 64, 128, 256])), int(r.integers(1, 12)), int(r.integers(1, 90))
