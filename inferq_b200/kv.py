@@ -131,8 +131,6 @@ class KvCache:
 
     def _new(self, shape, dtype, stream):
         """Memory of the stream that writes it; the current one may read it."""
-        if stream is None:
-            return torch.empty(shape, dtype=dtype, device=self.device)
         with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=self.device)):
             x = torch.empty(shape, dtype=dtype, device=self.device)
         if x.numel():
@@ -164,7 +162,11 @@ class KvCache:
         rows behind the last sequence are left as they are in ``out``."""
         if out is None:
             shape = (rows, self.kv_heads, self.head_dim)
-            out = self._new(shape, dtype, stream), self._new(shape, dtype, stream)
+            if stream is None:
+                out = (torch.empty(shape, dtype=dtype, device=self.device),
+                       torch.empty(shape, dtype=dtype, device=self.device))
+            else:
+                out = self._new(shape, dtype, stream), self._new(shape, dtype, stream)
         k, v = out
         if k.shape != v.shape or k.dtype != v.dtype or k.shape[0] != rows:
             raise ValueError("keys and values must have one shape and type, and the batch's rows")
@@ -180,7 +182,9 @@ class KvCache:
         a = self._rows("queries", q, 0, batch)
         rows, heads, _ = q.shape
         if out is None:
-            out = self._new((rows, heads, self.head_dim), q.dtype, stream)
+            # (empty_like: a microsecond less than torch.empty)
+            out = (torch.empty_like(q, memory_format=torch.contiguous_format) if stream is None else
+                   self._new(q.shape, q.dtype, stream))
         elif out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError("queries and outputs must have one shape and type")
         b = self._rows("outputs", out, heads, batch)
@@ -192,7 +196,7 @@ class KvCache:
         _lib.check(self._lib.iq_kv_attend_workspace(self._h, c, at, need))
         ws, n = None, need.value
         if n:
-            ws = self._new(n, torch.uint8, stream)
+            ws = q.new_empty(n, dtype=torch.uint8) if stream is None else self._new(n, torch.uint8, stream)
         _lib.check(self._lib.iq_kv_attend(self._h, c, at, *a, *b, None if ws is None else ws.data_ptr(), n,
                                           self._stream(stream)))
         return out
