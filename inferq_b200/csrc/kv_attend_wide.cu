@@ -12,11 +12,13 @@
 // its 4 KB a step would hold the 64-column product to two thirds of the
 // tensor rate (128 bytes a cycle; measured, with four score buffers in the
 // room that it leaves: 2048 bf16 rows over 32768 f16 tokens of hd 256 in 1315
-// us instead of 1140).  TMEM: O in hd columns, two buffers of S
-// (64 columns each; P replaces S in place), Q.  K tiles are K-major and V
-// tiles MN-major in the 128-byte swizzle, in which the f16 cache already
-// keeps its pages: its tiles arrive by bulk copies alone.  i8 tiles arrive as
-// bytes in small stages, and eight warps expand them to f16 integers.
+// us instead of 1140).  TMEM: O in hd columns, the buffers of S (64 columns
+// each; P replaces S in place), Q.  Of S there is room for two buffers at hd
+// 256 and four below, where scores then run three tiles ahead of the sums (two
+// and four, hd 128: 1035 and 930 us).  K tiles are K-major and V tiles MN-major
+// in the 128-byte swizzle, in which the f16 cache already keeps its pages: its
+// tiles arrive by bulk copies alone.  i8 tiles arrive as bytes in small stages,
+// and eight warps expand them to f16 integers.
 //
 // f32 rows enter as two f16 parts: Q's second part is a shared-memory operand
 // of a second product into the same S, P's second part lies beside the first.
@@ -42,8 +44,8 @@
 //
 // Bound: the chain scores -> softmax -> values of a tile, of which two are in
 // flight (tensor pipe active half of the cycles, issue slots 45%).  2048 bf16
-// rows of 16 heads over 32768 tokens of 2 heads of 256, unsplit: f16 1140 us
-// (930 TFLOP/s, 56% of a measured GEMM's rate), i8 1441 us; hd 128 539 us.
+// rows of 16 heads over 32768 tokens of 2 heads of 256, unsplit: f16 1130 us
+// (942 TFLOP/s, 57% of a measured GEMM's rate), i8 1405 us; hd 128 930 us.
 #include <cfloat>
 #include <climits>
 #include <type_traits>
@@ -80,9 +82,10 @@ struct Geo {
   static constexpr int kSmem = (kRing + kRingV) * kTileBytes + kQlo + 2 * kStages * kStage + kScaleBytes + 1024;
   static constexpr int kExpandWarps = FMT == kKvI8 ? 8 : 0;
   static constexpr int kThreads = (kExpandWarp + kExpandWarps) * 32;
-  static constexpr uint32_t kTmemS = HD, kTmemQ = HD + 2 * kT;
-  static constexpr uint32_t kTmemCols = HD + 2 * kT + HD / 2 > 256 ? 512 : 256;
-  static_assert(HD + 2 * kT + HD / 2 <= 512, "O, S and Q fit the tensor memory");
+  static constexpr int kBufs = HD < 256 ? 4 : 2;  // of scores
+  static constexpr uint32_t kTmemS = HD, kTmemQ = HD + kBufs * kT;
+  static constexpr uint32_t kTmemCols = 512;
+  static_assert(kTmemQ + HD / 2 <= kTmemCols, "O, S and Q fit the tensor memory");
   static_assert(kRingV * kTileBytes >= kM * HD * 2 || (FMT == kKvI8 && kRing * kTileBytes >= kM * HD * 2), "Q is staged where tiles come later");
   static_assert(kStages >= (kStageTokens == kT ? 2 : 3) || FMT != kKvI8, "see the loader's turns");
   static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
@@ -212,8 +215,8 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
     kv_attend_wide_kernel(const __grid_constant__ KvAttnArgs a, const bool vec) {
   using G_ = Geo<HD, FMT, F32Q>;
   constexpr float kCut = cut_of(F32Q);
-  constexpr int R = G_::kRing, RV = G_::kRingV, TB = G_::kTileBytes, NS = G_::kStages, SB = G_::kStage;
-  __shared__ __align__(8) uint64_t kfull[R], kempty[R], vfull[RV], vempty[RV], sfull[2], pfull[2], odone, qfull, decided, drained;
+  constexpr int NB = G_::kBufs, R = G_::kRing, RV = G_::kRingV, TB = G_::kTileBytes, NS = G_::kStages, SB = G_::kStage;
+  __shared__ __align__(8) uint64_t kfull[R], kempty[R], vfull[RV], vempty[RV], sfull[NB], pfull[NB], odone[NB], qfull, decided[2], drained;
   __shared__ __align__(8) uint64_t scfull[kScaleRing], scempty[kScaleRing];
   __shared__ __align__(8) uint64_t stfull[2 * NS], stempty[2 * NS];  // stages of keys, then of values
   __shared__ uint32_t tmem_s;
@@ -270,9 +273,10 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
       bar_init(&vfull[s], FMT == kKvI8 ? 4 : 1);
       bar_init(&vempty[s], 1);
     }
-    for (int b = 0; b < 2; b++) {
+    for (int b = 0; b < NB; b++) {
       bar_init(&sfull[b], 1);
       bar_init(&pfull[b], 8);
+      bar_init(&odone[b], 1);
     }
     for (int s = 0; s < kScaleRing; s++) {
       bar_init(&scfull[s], 2);
@@ -282,9 +286,9 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
       bar_init(&stfull[s], 1);
       bar_init(&stempty[s], 4);
     }
-    bar_init(&odone, 1);
     bar_init(&qfull, kSoftWarps);
-    bar_init(&decided, 8);
+    bar_init(&decided[0], 8);
+    bar_init(&decided[1], 8);
     bar_init(&drained, 1);
     abort_s = 0;
     bar_init_fence();
@@ -417,11 +421,11 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
     for (int ti = sp.first; ti < sp.end; ti = sp.next(ti), it++) {
       if ((it & 1) != grp) continue;
       mine = it;
-      const int b = it & 1, sr = it % kScaleRing, t0 = ti * kT + 32 * half;
+      const int b = it % NB, sr = it % kScaleRing, t0 = ti * kT + 32 * half;
       const float* sc = scales + sr * (2 * kT + 4);
       // A wait that ran out is told to the pair's other warp at its barrier,
       // so that no warp is left in one.
-      ok = ok && wait(&scfull[sr], (it / kScaleRing) & 1) && wait(&sfull[b], (it >> 1) & 1);
+      ok = ok && wait(&scfull[sr], (it / kScaleRing) & 1) && wait(&sfull[b], (it / NB) & 1);
       tc_after();
       const uint32_t st = lanes + G_::kTmemS + b * kT;
       uint32_t s0[32];
@@ -451,7 +455,10 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
       for (int j = 4; j < 16; j++) m4[j & 3] = max3(m4[j & 3], x[j].x, x[j].y);
       float mx = fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]) * cq;
       if (it > 0) {  // the other group's decision on the tile before
-        ok = ok && wait(&decided, (it - 1) & 1);
+        // (A barrier for each group: scores lie ready for several tiles, so a warp
+        // may be at its next tile before its own group is through with this one;
+        // on one barrier it would meet a phase two behind.)
+        ok = ok && wait(&decided[(it - 1) & 1], ((it - 1) >> 1) & 1);
         const float mo = mrow[row];
         const int eo = erow[row];
         if (mo != m || eo != ev) {
@@ -489,7 +496,7 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
         }
       }
       __syncwarp();
-      if (lane == 0) bar_arrive(&decided);
+      if (lane == 0) bar_arrive(&decided[grp]);
       const float r = (m == -INFINITY ? 0.f : m) - 7.f + (float)ev;
       l2 = mul2(l2, make_float2(kCut, kCut));
       const float4* vs = reinterpret_cast<const float4*>(sc + kT + 32 * half);
@@ -526,7 +533,9 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
       __syncwarp();
       if (lane == 0) bar_arrive(&scempty[sr]);
       if (it > 0 && __any_sync(0xffffffffu, fo != 1.f)) {
-        ok = wait(&odone, (it - 1) & 1);  // the previous product has been added
+        // The previous product has been added.  (One phase behind at most: these
+        // scores came after the product of tile it - NB.)
+        ok = wait(&odone[(it - 1) % NB], ((it - 1) / NB) & 1);
         tc_after();
 #pragma unroll 1
         for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 16) {
@@ -630,7 +639,7 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
       if (!wait(&kfull[s], (i / R) & 1)) return false;
       tc_after();
       if (leader) {
-        const uint32_t d = tmem + G_::kTmemS + (i & 1) * kT, kb = k0 + s * TB;
+        const uint32_t d = tmem + G_::kTmemS + (i % NB) * kT, kb = k0 + s * TB;
         if constexpr (F32Q) {  // the small parts first: fewer cuts of the whole sum
 #pragma unroll
           for (int st = 0; st < HD / 16; st++)
@@ -640,30 +649,35 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
 #pragma unroll
         for (int st = 0; st < HD / 16; st++)
           mma_ts(d, tmem + G_::kTmemQ + 8 * st, sw128(kb + (st >> 2) * (kT * 128) + (st & 3) * 32, 16), dS, F32Q || st > 0);
-        commit(&sfull[i & 1]);
+        commit(&sfull[i % NB]);
         commit(&kempty[s]);
       }
       __syncwarp();
       return true;
     };
-    int it = 0, ti = sp.first;
-    if (ok && ti < sp.end) ok = score(0);
-    for (; ok && ti < sp.end; it++) {
-      ti = sp.next(ti);
-      if (ti < sp.end && !(ok = score(it + 1))) break;
+    // Scores run NB - 1 tiles ahead of the sums: product it - 1, issued before,
+    // has read the buffer that the scores of tile it + NB - 1 fill.
+    int ns = 0, ts = sp.first;
+#pragma unroll 1
+    for (; ok && ts < sp.end && ns < NB - 1; ts = sp.next(ts)) ok = score(ns++);
+    for (int it = 0; ok && it < ns; it++) {
+      if (ts < sp.end) {
+        ts = sp.next(ts);
+        if (!(ok = score(ns++))) break;
+      }
       const int s = it % RV;
-      ok = wait(&pfull[it & 1], (it >> 1) & 1) && wait(&vfull[s], (it / RV) & 1);
+      ok = wait(&pfull[it % NB], (it / NB) & 1) && wait(&vfull[s], (it / RV) & 1);
       if (!ok) break;
       tc_after();
       if (leader) {
-        const uint32_t pa = tmem + G_::kTmemS + (it & 1) * kT, vb = v0 + s * TB;
+        const uint32_t pa = tmem + G_::kTmemS + (it % NB) * kT, vb = v0 + s * TB;
 #pragma unroll
         for (int part = 0; part < (F32Q ? 2 : 1); part++)
 #pragma unroll
           for (int kk = 0; kk < kT / 16; kk++)
             mma_ts(tmem, pa + part * 32 + 8 * kk, sw128(vb + kk * 2048, kT * 128), dO, it > 0 || kk > 0 || part > 0);
         commit(&vempty[s]);
-        commit(&odone);
+        commit(&odone[it % NB]);
       }
       __syncwarp();
     }

@@ -118,3 +118,18 @@ def test_windows_first_tokens_and_splits_past_any_table(cuda, rows, fmt, dtype):
     for chunk in (64, most - 63):
         close(s.cache.attend(q, b, window=7, sinks=0, chunk=chunk), *s.want(window=7), s.dt)
     s.cache.status()
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd", [(32, 8, 128), (8, 2, 64), (16, 2, 256)])
+@pytest.mark.parametrize("fmt,dtype", [("f16", "f16"), ("i8", "f32"), ("i8", "bf16")])
+def test_cold_and_warm_calls_agree(cuda, heads, kv_heads, hd, fmt, dtype):
+    """Bit for bit, whatever order copies and warps happen to run in: caches emptied before every call."""
+    s = Sequences([(300, 3000), (41, 700), (90, 60)], heads=heads, kv_heads=kv_heads, hd=hd, fmt=fmt, dtype=dtype)
+    q, b = s.q.cuda(), s.batch()
+    flush = torch.empty(200 << 20, dtype=torch.uint8, device="cuda")
+    for kw in ({}, {"window": 1023, "sinks": 5}, {"chunk": 512}):
+        want = s.cache.attend(q, b, **kw)
+        for i in range(15):
+            flush.fill_(i)
+            assert torch.equal(s.cache.attend(q, b, **kw), want), (kw, i)
+    s.cache.status()
