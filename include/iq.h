@@ -364,8 +364,9 @@ typedef struct iq_kv_batch {
 } iq_kv_batch;
 
 /* Errors as elsewhere; what only the device can see (a position outside the
- * table, a page id outside the pool) skips the row or token and is reported
- * by iq_kv_status.  Calls are enqueued on `stream` (NULL: the legacy stream)
+ * table, a page id outside the pool) skips the row or token (in attention, the
+ * rows that would see it have undefined results, the others their own) and is
+ * reported by iq_kv_status.  Calls are enqueued on `stream` (NULL: the legacy stream)
  * of the cache's device, may be captured, and allocate nothing. */
 int iq_kv_create(int format, int kv_heads, int head_dim, int page_tokens, int64_t pages, iq_kv** out);
 /* (No call on the cache may still be running.) */

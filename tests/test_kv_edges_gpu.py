@@ -133,3 +133,21 @@ def test_cold_and_warm_calls_agree(cuda, heads, kv_heads, hd, fmt, dtype):
             flush.fill_(i)
             assert torch.equal(s.cache.attend(q, b, **kw), want), (kw, i)
     s.cache.status()
+
+
+@pytest.mark.parametrize("rows", [1, 4, 70])
+@pytest.mark.parametrize("fmt", ["i8", "f16"])
+def test_a_bad_page_id_is_the_matter_of_the_rows_that_see_it(cuda, fmt, rows):
+    s = Sequences([(rows, 30), (rows, 300)], fmt=fmt, page=64)
+    q, b = s.q.cuda(), s.batch()
+    want = s.cache.attend(q, b)
+    s.table[1, 3] = 2**31 - 1
+    got = s.cache.attend(q, b)
+    with pytest.raises(_lib.IqError, match="pool"):
+        s.cache.status()
+    assert torch.equal(got[:rows], want[:rows])
+    s.table[1, 3] = -7
+    s.cache.attend(q, b)
+    with pytest.raises(_lib.IqError, match="pool"):
+        s.cache.status()
+    s.cache.status()
