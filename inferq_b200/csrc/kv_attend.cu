@@ -9,9 +9,10 @@
 // bits or f16, a and b f32), so the matrix instructions multiply K and V as
 // they are stored, a_t scales the score and b_t the weight:
 //     s_t = a_t (q . K_t),  o = sum_t (p_t b_t) V_t / l.
-// Weights enter as f16: p_t b_t 2^(14 - e), with 2^e above every b met so far
-// (e grows like m; the accumulators follow by powers of two), so the largest
-// weights are at most 2^14 and weights down to 2^-28 of them keep 11 bits.
+// Weights enter as f16: p_t b_t 2^(14 - e), with 2^e above every b that the row
+// has seen so far (e grows like m, a row's own; the accumulators follow by
+// powers of two), so the largest weights are at most 2^14 and weights down to
+// 2^-28 of them keep 11 bits.
 // f32 rows split queries and weights into two f16 parts each (22 bits).  A
 // query row is divided by a power of two first, which joins its scale.
 //
@@ -110,13 +111,18 @@ struct Geo {
   static constexpr int kQld = HD * 2 + 16;                                // bytes of a staged query row
   static constexpr int kQBytes = kTQ * kQld * (F32Q ? 2 : 1);
   static constexpr int kPBytes = NT * 4 * 32 * 8 * (F32Q ? 2 : 1);
-  static_assert(kGeo.fixed == kQBytes + kPBytes + 6 * kTQ * 4 + 64, "queries, weights, maxima, factors, positions");
+  static_assert(kGeo.fixed == kQBytes + kPBytes + 12 * kTQ * 4 + 64, "queries, weights, maxima, factors, positions, exponents");
   static constexpr int kStages = kGeo.stages, kSmem = kGeo.smem;
   static_assert(kStages >= 2, "two stages keep a copy in flight");
 };
 
+// CTAs an SM that registers must allow: those for which they suffice without
+// spills (five warps of up to 168 registers: two).
 template <int HD, int FMT, int NT, bool F32Q>
-__global__ void __launch_bounds__(160, NT == 1 ? 3 : 1) kv_attend_kernel(const __grid_constant__ KvAttnArgs a, const bool vec) {
+constexpr int kMinCtas = NT == 1 ? 3 : (HD == 64 && NT == 4) || (HD == 256 && NT == 2 && FMT == kKvI8 && !F32Q) ? 2 : 1;
+
+template <int HD, int FMT, int NT, bool F32Q>
+__global__ void __launch_bounds__(160, kMinCtas<HD, FMT, NT, F32Q>) kv_attend_kernel(const __grid_constant__ KvAttnArgs a, const bool vec) {
   using G_ = Geo<HD, FMT, NT, F32Q>;
   constexpr int TQ = G_::kTQ, ST = G_::kStages, QLD = G_::kQld;
   __shared__ __align__(8) uint64_t full[ST], empty[ST];
@@ -128,7 +134,9 @@ __global__ void __launch_bounds__(160, NT == 1 ? 3 : 1) kv_attend_kernel(const _
   float* mx = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(ps) + G_::kPBytes);  // [4][TQ]
   float* cq = mx + 4 * TQ;                                                   // [TQ] row factor
   int* rpos = reinterpret_cast<int*>(cq + TQ);                               // [TQ] row position, -1: none
-  int* evw = rpos + TQ;                                                      // [4]
+  int* evr = rpos + TQ;                                                      // [4][TQ] exponents of a masked tile
+  float2* esc = reinterpret_cast<float2*>(evr + 4 * TQ);                     // [TQ] {factor of the sums, of the scales}
+  int* evw = reinterpret_cast<int*>(esc + TQ);                               // [4] exponent of a tile
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const KvPool& p = a.pool;
@@ -265,7 +273,12 @@ __global__ void __launch_bounds__(160, NT == 1 ? 3 : 1) kv_attend_kernel(const _
   float mrow[NT][2], l[NT][2];
 #pragma unroll
   for (int n = 0; n < NT; n++) mrow[n][0] = mrow[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.f;
-  int ev = -100;  // so that 2^(14 - ev) is finite
+  // Rows have one exponent, evu, until a masked tile: then each has its own,
+  // kept by thread r for row r and at most evu, until a whole tile reaches evu.
+  // (Every row's in every thread's registers: spills, and 25% more time for 64
+  // f32 rows of hd 256.)
+  int evu = -100, mine = -100;  // so that 2^(14 - e) is finite
+  bool one = true;
   bool failed = false;
 
   int it = 0;
@@ -338,27 +351,67 @@ __global__ void __launch_bounds__(160, NT == 1 ? 3 : 1) kv_attend_kernel(const _
           m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
           if (lane < 4) mx[warp * TQ + q] = m;
         }
-      // exponent above the tile's value scales
+      // Exponent above the tile's value scales, and in a masked tile above those
+      // that a row sees: a hidden token's would take bits of the row's weights.
       uint32_t vb = 0;
       if (lane < 16 && t0 + 16 * warp + lane < sp.tokens) vb = __float_as_uint(sc[64 + 16 * warp + lane]);
       if (vb >= 0x7f800000u) vb = 0;  // a NaN scale's rows are NaN whatever the exponent
       vb = __reduce_max_sync(0xffffffffu, vb);
       if (lane == 0) evw[warp] = max((int)(vb >> 23), 1) - 126;
+      if (!whole) {
+        uint32_t e0 = __float_as_uint(sc[64 + 16 * warp + g]) >> 23, e1 = __float_as_uint(sc[64 + 16 * warp + g + 8]) >> 23;
+        if (e0 >= 255) e0 = 0;
+        if (e1 >= 255) e1 = 0;
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+          const int q = n * 8 + 2 * t;
+          uint32_t x = 0;  // the two rows' in halves of a word
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const int rp = rpos[q + e];
+            x |= max(sp.sees(rp, ta) ? e0 : 0, sp.sees(rp, ta + 8) ? e1 : 0) << (16 * e);
+          }
+          x = __vmaxu2(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          x = __vmaxu2(x, __shfl_xor_sync(0xffffffffu, x, 8));
+          x = __vmaxu2(x, __shfl_xor_sync(0xffffffffu, x, 16));
+          if (lane < 4) {
+            evr[warp * TQ + q] = max((int)(x & 0xffff), 1) - 126;
+            evr[warp * TQ + q + 1] = max((int)(x >> 16), 1) - 126;
+          }
+        }
+      }
     }
     if (consumers_any(!ok)) {
       failed = true;
       break;
     }
     // -------------------------------------------------- weights and sums
-    const int evn = max(max(ev, max(evw[0], evw[1])), max(evw[2], evw[3]));
-    const float shrink = ev - evn < -126 ? 0.f : pow2i(ev - evn);
-    const float up = pow2i(-evn) * 16384.f;
-    ev = evn;
-    const float v0 = sc[64 + 16 * warp + g] * up, v1 = sc[64 + 16 * warp + g + 8] * up;
+    const int evt = max(max(evw[0], evw[1]), max(evw[2], evw[3]));
+    const float b0 = sc[64 + 16 * warp + g], b1 = sc[64 + 16 * warp + g + 8];
+    const bool whole = sp.whole(t0, kTile), own = !(whole && one);
+    auto shrink_of = [](int from, int to) { return from - to < -126 ? 0.f : pow2i(from - to); };
+    float shrink = 0.f, up = 0.f;  // of all rows
+    if (own) {
+      if (threadIdx.x < TQ) {
+        const int r = threadIdx.x, from = one ? evu : mine;
+        mine = max(from, whole ? evt : max(max(evr[r], evr[TQ + r]), max(evr[2 * TQ + r], evr[3 * TQ + r])));
+        esc[r] = make_float2(shrink_of(from, mine), pow2i(14 - mine));
+      }
+      consumers_sync();
+      one = whole && evt >= evu;
+      evu = max(evu, evt);
+    } else {
+      const int to = max(evu, evt);
+      shrink = shrink_of(evu, to);
+      up = pow2i(14 - to);
+      evu = to;
+    }
     float fo[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
       float w[4];
+      float4 f = make_float4(shrink, up, shrink, up);
+      if (own) f = *reinterpret_cast<const float4*>(esc + n * 8 + 2 * t);  // of both rows
 #pragma unroll
       for (int e = 0; e < 2; e++) {
         const int q = n * 8 + 2 * t + e;
@@ -368,10 +421,10 @@ __global__ void __launch_bounds__(160, NT == 1 ? 3 : 1) kv_attend_kernel(const _
         mrow[n][e] = m;
         const float p0 = ex2(sa[n][e] - ms), p1 = ex2(sa[n][2 + e] - ms);
         l[n][e] = l[n][e] * alpha + (p0 + p1);
-        fo[n][e] = alpha * shrink;
+        fo[n][e] = alpha * (e ? f.z : f.x);
         // a hidden token weighs zero whatever its scale is
-        w[e] = sa[n][e] == -INFINITY ? 0.f : p0 * v0;
-        w[2 + e] = sa[n][2 + e] == -INFINITY ? 0.f : p1 * v1;
+        w[e] = sa[n][e] == -INFINITY ? 0.f : p0 * (b0 * (e ? f.w : f.y));
+        w[2 + e] = sa[n][2 + e] == -INFINITY ? 0.f : p1 * (b1 * (e ? f.w : f.y));
       }
       const uint32_t h0 = pack2(w[0], w[1]), h1 = pack2(w[2], w[3]);
       ps[(n * 4 + warp) * 32 + lane] = make_uint2(transpose8(h0), transpose8(h1));
@@ -447,7 +500,8 @@ __global__ void __launch_bounds__(160, NT == 1 ? 3 : 1) kv_attend_kernel(const _
     return;
   }
   // ------------------------------------------------------------- results
-  consumers_sync();  // mx is read no more
+  consumers_sync();  // mx and esc are read no more
+  if (threadIdx.x < TQ) esc[threadIdx.x].x = pow2i(one ? evu : mine);
 #pragma unroll
   for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -459,7 +513,6 @@ __global__ void __launch_bounds__(160, NT == 1 ? 3 : 1) kv_attend_kernel(const _
       if (lane < 4) mx[warp * TQ + n * 8 + 2 * t + e] = v;
     }
   consumers_sync();
-  const float back = pow2i(ev);
 #pragma unroll
   for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -469,6 +522,7 @@ __global__ void __launch_bounds__(160, NT == 1 ? 3 : 1) kv_attend_kernel(const _
       const float sum = (mx[q] + mx[TQ + q]) + (mx[2 * TQ + q] + mx[3 * TQ + q]);
       const int row = tr.row0 + rr / group, h = kvh * group + rr % group;
       const int64_t rh = (int64_t)row * a.heads + h;
+      const float back = esc[q].x;
       const float f = a.slots > 1 ? 0x1p-14f : sum != 0.f ? __fdiv_rn(0x1p-14f, sum) : 0.f;
       if (a.slots > 1 && warp == 0 && g == 0) a.ml[rh * a.slots + slot] = make_float2(mrow[n][e], sum);
       if (!sums) continue;

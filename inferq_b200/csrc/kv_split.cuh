@@ -161,7 +161,7 @@ struct KvNarrow {
 constexpr KvNarrow kv_narrow(int format, int hd, int nt, bool f32) {
   const int tile = kKvTile * hd * (format == kKvI8 ? 1 : 2), per = 2 * tile + 512, parts = f32 ? 2 : 1;
   KvNarrow g = {};
-  g.fixed = 8 * nt * (hd * 2 + 16) * parts + nt * 1024 * parts + 6 * 8 * nt * 4 + 64;
+  g.fixed = 8 * nt * (hd * 2 + 16) * parts + nt * 1024 * parts + 12 * 8 * nt * 4 + 64;
   const int limit = 2 * tile > 32768 ? 226 : g.fixed <= 10 * 1024 ? 78 : g.fixed <= 48 * 1024 ? 112 : 226;
   const int room = limit * 1024 - 2048 - g.fixed;
   g.stages = room / per > 4 ? 4 : room / per;
