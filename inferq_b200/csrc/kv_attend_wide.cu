@@ -29,8 +29,9 @@
 // decides on it (after the group of tile i - 1 has), and it moves only when a
 // tile exceeds it by more than 2^8 (one barrier a tile says whether any row of
 // a pair of warps needs that; the accumulator is then rescaled in TMEM).  With
-// m the maximum and ev two binades above the first value scales, a row's
-// reference is r = m - 7 + ev:
+// m the maximum and ev two binades above the first value scales that the row
+// sees (all of a tile's, or in a masked tile its own), a row's reference is
+// r = m - 7 + ev:
 //     p_t = 2^(s_t log2e - r),  weight p_t b_t <= 2^8 2^7 2^-ev b_t <= 2^15,
 // the weight of the largest score about 2^4, and f16 keeps 11 bits down to
 // 2^-14 and 2^-25 below.  {r, l, o} are the partial result.
@@ -236,6 +237,7 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
   float* mrow = tops + 2 * kM;                       // [row] maximum
   int* erow = reinterpret_cast<int*>(mrow + kM);     // [row] exponent
   float* sums = reinterpret_cast<float*>(erow + kM); // [2][row]
+  int* eshare = reinterpret_cast<int*>(sums);        // the halves' exponents, before the sums
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const KvPool& p = a.pool;
@@ -432,7 +434,7 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
       tmem_ld32(st + 32 * half, s0);
       float2 x[16];
       const float4* ks = reinterpret_cast<const float4*>(sc + 32 * half);
-      const int et = __float_as_int(sc[2 * kT]);
+      int et = __float_as_int(sc[2 * kT]);
       tmem_wait(s0);
 #pragma unroll
       for (int j = 0; j < 8; j++) {
@@ -447,6 +449,19 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
           if (!sp.sees(rp, t0 + 2 * j)) x[j].x = -INFINITY;
           if (!sp.sees(rp, t0 + 2 * j + 1)) x[j].y = -INFINITY;
         }
+        // The exponent above the scales that the row sees: a hidden token's would
+        // take bits of its weights.
+        const float4* vs = reinterpret_cast<const float4*>(sc + kT + 32 * half);
+        float top = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const float4 v = vs[j];
+          if (x[2 * j].x != -INFINITY && v.x < INFINITY) top = fmaxf(top, v.x);
+          if (x[2 * j].y != -INFINITY && v.y < INFINITY) top = fmaxf(top, v.y);
+          if (x[2 * j + 1].x != -INFINITY && v.z < INFINITY) top = fmaxf(top, v.z);
+          if (x[2 * j + 1].y != -INFINITY && v.w < INFINITY) top = fmaxf(top, v.w);
+        }
+        et = max(__float_as_int(top) >> 23, 1) - 126;
       }
       float m4[4];
 #pragma unroll
@@ -469,20 +484,22 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
         }
       }
       // both threads of a row have read its scores when the barrier opens
-      const bool move = mx > m + 8.f || m == -INFINITY;
-      const int en = et > ev ? et + 2 : ev;
+      int en = ev;
+      const bool move = mx > m + 8.f || m == -INFINITY || et > ev;
       float fo = 1.f;
-      if (pair_any(pair, move || !ok) || en != ev) {
+      if (!whole || pair_any(pair, move || !ok)) {
         tops[half * kM + row] = mx;
-        sums[half * kM + row] = ok ? 0.f : 1.f;
+        eshare[half * kM + row] = ok ? et : INT_MAX;  // INT_MAX: the warp gave up
         pair_sync(pair);
         mx = fmaxf(mx, tops[(half ^ 1) * kM + row]);
-        const bool other = sums[(half ^ 1) * kM + row] == 0.f;
+        const int eo = eshare[(half ^ 1) * kM + row];
         pair_sync(pair);
-        if (!__all_sync(0xffffffffu, ok && other)) {
+        if (!__all_sync(0xffffffffu, ok && eo != INT_MAX)) {
           ok = false;
           break;
         }
+        et = max(et, eo);
+        if (et > ev) en = et + 2;
         const float mn = mx > m + 8.f || m == -INFINITY ? mx : m;
         // o and l by 2^(old reference - new)
         const float d = (m == -INFINITY ? 0.f : m) - (mn == -INFINITY ? 0.f : mn) + (float)(ev - en);

@@ -77,6 +77,48 @@ def test_short_rows_are_the_same_whatever_their_window_hides(cuda, fmt, dtype, h
         s.v = keep
 
 
+CHUNKS = [("i8", "f32", 16, 256), ("f16", "f32", 16, 64), ("f16", "f32", 16, 128), ("f16", "bf16", 16, 256), ("i8", "bf16", 16, 128),
+          ("i8", "f32", 16, 64), ("f16", "bf16", 32, 64)]
+
+
+@pytest.mark.parametrize("binades", [1, 12, 45, 100])
+@pytest.mark.parametrize("fmt,dtype,heads,hd", CHUNKS)
+def test_chunks_are_the_same_whatever_stands_behind_their_rows(cuda, fmt, dtype, heads, hd, binades):
+    """Row r's successor holds the large value: rows up to r keep their bits."""
+    s = Sequences([(70, 190)], heads=heads, hd=hd, fmt=fmt, dtype=dtype, spread=5.0, seed=binades)
+    q, b = s.q.cuda(), s.batch()
+    want, most = s.want()
+    before = s.cache.attend(q, b)
+    keep = s.v
+    for r in (0, 5, 14, 40, 68):
+        rewrite(s, {190 + r + 1: 2.0 ** binades})
+        got = s.cache.attend(q, b)
+        assert torch.equal(got[:r + 1], before[:r + 1]), r
+        near(s, got[:r + 1], want[:r + 1], most[:r + 1], r)
+        s.v = keep
+    s.cache.status()
+
+
+@pytest.mark.parametrize("binades", [1, 12, 45, 100])
+@pytest.mark.parametrize("fmt,dtype,heads,hd", CHUNKS)
+def test_chunks_are_the_same_whatever_their_window_hides(cuda, fmt, dtype, heads, hd, binades):
+    """Token t leaves the window of the rows from t + window on."""
+    s = Sequences([(70, 190)], heads=heads, hd=hd, fmt=fmt, dtype=dtype, spread=5.0, seed=binades)
+    q, b, kw = s.q.cuda(), s.batch(), {"window": 33, "sinks": 3}
+    want, most = s.want(**kw)
+    before = s.cache.attend(q, b, **kw)
+    keep = s.v
+    for token in (3, 64, 157, 170, 215):
+        rewrite(s, {token: 2.0 ** binades})
+        got = s.cache.attend(q, b, **kw)
+        first = max(0, token + 33 - 190)  # rows from here on do not see it
+        assert torch.equal(got[first:], before[first:]), token
+        near(s, got[first:], want[first:], most[first:], token)
+        rows = max(0, token - 190)  # nor do the rows before it
+        assert torch.equal(got[:rows], before[:rows]), token
+        s.v = keep
+
+
 @pytest.mark.parametrize("kv", ["f16", "i8"])
 def test_verify_rows_equal_sequential_rows_bitwise_where_scores_spread(cuda, kv):
     """The queries' norm weighs eight times as much: scores lie some 10 nats
