@@ -249,6 +249,8 @@ inline size_t kv_plan(KvAttnArgs& a, int max_rows) {
       if (n > 1) cost += 3 + slots * result;
       if (!a.chunk || cost < best) best = cost, a.chunk = (int)chunk;
     }
+    // (the steps of n may pass over `most`, every split before it too long for one accumulator)
+    if (!a.chunk) a.chunk = f32 ? kWideChunkF32 : kWideChunk;
   }
   if (tq == 128) a.chunk = std::min(a.chunk, a.dtype == F32 ? kWideChunkF32 : kWideChunk);
   const int64_t all = std::max<int64_t>(ceil_div(cap, a.chunk), 1);
