@@ -402,7 +402,7 @@ int iq_kv_read(const iq_kv* c, const iq_kv_batch* b, int dtype, void* k, int64_t
  * a sequence and KV head (max_rows * heads / kv_heads), a row's result
  * depends on its own context and chunk only, bit for bit.  More query rows
  * run on the tcgen05 tensor cores (from 17, where the call chooses the
- * chunk), where a split is at most 1536 tokens for IQ_F32 and 32768
+ * chunk), where a split is at most 640 tokens for IQ_F32 and 16384
  * otherwise: longer ones are cut to that, since the accumulators round
  * towards zero. */
 typedef struct iq_kv_attn {

@@ -36,6 +36,13 @@
 // the weight of the largest score about 2^4, and f16 keeps 11 bits down to
 // 2^-14 and 2^-25 below.  {r, l, o} are the partial result.
 //
+// The tensor cores cut a sum off towards zero at every instruction, eight of
+// them a tile for f32 rows and four for others, while l is summed by rounding
+// additions.  What O loses depends on what is added (nothing behind a first
+// token that outweighs the rest, up to 5e-8 of it an instruction where equal
+// values add up), so no factor on l makes up for it; the length of a chunk
+// bounds it instead (kv_split.cuh), and the join adds by rounding.
+//
 // Warps: 0-15 softmax and results, 16 issues the MMAs (one elected lane: issued
 // under a plain lane test each instruction cost four times the cycles), 17-20
 // request keys and values (two warps each, tiles in turn: a tile costs one some
@@ -203,19 +210,10 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 __device__ __forceinline__ float2 unpack2(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 
-// The tensor cores cut a sum off towards zero at every step; of an accumulator
-// that many tiles go into, 3.3e-8 a step is lost on average (measured: 1.8e-5
-// over 8192 tokens of f32 rows, 6.8e-5 over 32768).  The sum of the weights
-// loses as much, so that the mean of it leaves the quotient; what a single
-// element loses more or less than the mean is bounded by the length of a chunk
-// (kv_split.cuh).  Steps of two tiles: a group has every other one.
-constexpr float cut_of(bool f32) { return 1.f - 2 * (f32 ? 8 : 4) * 3.3e-8f; }
-
 template <int HD, int FMT, bool F32Q>
 __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
     kv_attend_wide_kernel(const __grid_constant__ KvAttnArgs a, const bool vec) {
   using G_ = Geo<HD, FMT, F32Q>;
-  constexpr float kCut = cut_of(F32Q);
   constexpr int NB = G_::kBufs, R = G_::kRing, RV = G_::kRingV, TB = G_::kTileBytes, NS = G_::kStages, SB = G_::kStage;
   __shared__ __align__(8) uint64_t kfull[R], kempty[R], vfull[RV], vempty[RV], sfull[NB], pfull[NB], odone[NB], qfull, decided[2], drained;
   __shared__ __align__(8) uint64_t scfull[kScaleRing], scempty[kScaleRing];
@@ -515,7 +513,6 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
       __syncwarp();
       if (lane == 0) bar_arrive(&decided[grp]);
       const float r = (m == -INFINITY ? 0.f : m) - 7.f + (float)ev;
-      l2 = mul2(l2, make_float2(kCut, kCut));
       const float4* vs = reinterpret_cast<const float4*>(sc + kT + 32 * half);
 #pragma unroll
       for (int hh = 0; hh < 2; hh++) {

@@ -190,10 +190,13 @@ inline int64_t kv_tiles_bound(const KvAttnArgs& a, int tq) {
 }
 
 // The most tokens that one accumulator of the tensor-core kernel sums, for the
-// cuts that its steps make (kv_attend_wide.cu).  f32 rows: relative error
-// 1.0e-6 over 640 tokens, 3.0e-6 over 2560, 9.4e-6 over 8192 (32-bit torch
-// operations: 1.4e-6); 16-bit rows' own rounding covers 32768 tokens' cuts.
-constexpr int kWideChunkF32 = 1536, kWideChunk = 32768;
+// cuts that its steps make (kv_attend_wide.cu).  f32 rows over 640 tokens:
+// 4.0e-6 where equal values add up, 2.0e-6 of the outputs' size for values of
+// both signs (over 1536: 1.0e-5 and 4.0e-6; 32-bit torch operations 1.4e-6);
+// 512 of them over 2560 tokens take 78 us instead of 63, 2048 over 32768 3300
+// instead of 2584.  16-bit rows over 16384 tokens: 5.5e-5, an eighth of f16's
+// half step; 2048 over 131072 i8 tokens 5690 us instead of 5470.
+constexpr int kWideChunkF32 = 640, kWideChunk = 16384;
 
 // Fills tq, chunk (where it is 0) and slots; the workspace bytes.
 inline size_t kv_plan(KvAttnArgs& a, int max_rows) {
@@ -207,6 +210,8 @@ inline size_t kv_plan(KvAttnArgs& a, int max_rows) {
   a.chunk = std::min(a.chunk, end);
   const int tile_tokens = (tq - 1) / group + 1;
   const int64_t span = a.window ? std::min<int64_t>(cap, (int64_t)a.window + a.sinks + tile_tokens + kKvTile) : cap;
+  // what one accumulator may sum; a window's rows see no more than `span` tokens of any chunk
+  const int64_t limit = tq != 128 ? span : a.dtype == F32 ? kWideChunkF32 : kWideChunk;
   if (!a.chunk) {
     // The split n with the least estimated time, in us: CTAs run in waves of
     // `ctas` an SM; a wave costs its tiles, at the SM's share of what bounds
@@ -235,7 +240,7 @@ inline size_t kv_plan(KvAttnArgs& a, int max_rows) {
     for (int64_t n = 1; n <= most; n += 1 + n / 16) {
       // (unsplit, a chunk holds all of the table: first tokens and window in one)
       const int64_t chunk = align_up(n == 1 ? std::max<int64_t>(cap, 1) : ceil_div(span, n), kKvTile);
-      if (wide && chunk > (f32 ? kWideChunkF32 : kWideChunk) && n < most) continue;
+      if (std::min(chunk, span) > limit && n < most) continue;
       const int64_t slots = n == 1 ? 1 : ceil_div(span, chunk) + (a.window && a.sinks ? 1 : 0);
       const int64_t all = items * slots, full = all / (sms * ctas), rest = all % (sms * ctas);
       const double tiles = (double)ceil_div(ceil_div(span, n), kKvTile);
@@ -250,9 +255,9 @@ inline size_t kv_plan(KvAttnArgs& a, int max_rows) {
       if (!a.chunk || cost < best) best = cost, a.chunk = (int)chunk;
     }
     // (the steps of n may pass over `most`, every split before it too long for one accumulator)
-    if (!a.chunk) a.chunk = f32 ? kWideChunkF32 : kWideChunk;
+    if (!a.chunk) a.chunk = (int)limit;
   }
-  if (tq == 128) a.chunk = std::min(a.chunk, a.dtype == F32 ? kWideChunkF32 : kWideChunk);
+  if (span > limit) a.chunk = (int)std::min<int64_t>(a.chunk, limit);
   const int64_t all = std::max<int64_t>(ceil_div(cap, a.chunk), 1);
   a.slots = (int)all;
   if (a.window)
