@@ -248,7 +248,9 @@ typedef struct iq_verify_result {
  * draft prefix, rolls the DeltaNet state back to the committed boundary and
  * truncates the KV cache (QuantizedModelState::rollback,
  * quantized_model.rs:177-204) -- all before the single host synchronization.
- * logits [rows][vocab] / hidden [rows][hidden] are optional host outputs. */
+ * logits [rows][vocab] / hidden [rows][hidden] are optional host outputs.
+ * After IQ_ETIMEDOUT (here or from iq_forward) the rows of that pass are
+ * invalid but counted in the position: reset the state or import an image. */
 int iq_verify(iq_state* s, const uint32_t* tokens, int rows, iq_verify_result* out, float* logits, float* hidden);
 
 /* Roll the last iq_forward pass back to its first `committed_rows` rows
@@ -267,7 +269,8 @@ int iq_rollback(iq_state* s, int committed_rows);
  * committed tokens, token i paired with the target's normalized hidden row
  * of the position before it: `prev_hidden` (H floats) for the first, NULL
  * only at position 0 (zeros), then rows 0..rows-2 of `target_hidden`
- * ([rows][H], host).  No logits.
+ * ([rows][H], host).  No logits.  After IQ_ETIMEDOUT the cache stands at
+ * `position`, and the call can be made again.
  */
 int iq_mtp_sync(iq_state* s, int64_t position, const float* prev_hidden, const uint32_t* tokens, int rows,
                 const float* target_hidden);
@@ -287,7 +290,8 @@ int iq_mtp_shifted_inputs(const float* prev_hidden, const float* target_hidden, 
  * (probs, margins may be NULL); *n is the number of leading drafts whose
  * top-1 probability is >= min_conf (draft_mtp stops before the first that is
  * not).  Stop tokens are the caller's, as in the reference.  The MTP cache
- * advances by `depth`; the next iq_mtp_sync truncates it. */
+ * advances by `depth`; the next iq_mtp_sync truncates it.  After IQ_ETIMEDOUT
+ * it has not advanced. */
 int iq_mtp_draft(iq_state* s, uint32_t seed, const float* hidden, int depth, int draft_vocab, float min_conf,
                  uint32_t* tokens, float* probs, float* margins, int* n);
 

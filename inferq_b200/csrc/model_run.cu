@@ -1060,22 +1060,41 @@ int alloc_state(iq_state* s) {
   return build_plans(s);
 }
 
+// The status of the passes enqueued so far, read with the stream's next
+// synchronization (run_pass has these copies in its graph).
+int fetch_device_waits(iq_state* s) {
+  if (int* f = qmv_timeout_flag()) IQ_CUDA(cudaMemcpyAsync(s->h_result + 4, f, sizeof(int), cudaMemcpyDeviceToHost, s->st));
+  if (s->kv_format)
+    IQ_CUDA(cudaMemcpyAsync(s->h_result + 5, s->kv_flag.p, sizeof(int), cudaMemcpyDeviceToHost, s->st));
+  return IQ_OK;
+}
+
 // After a synchronized pass: a GEMV that gave up waiting for its weights
-// (bounded wait) fails the call with IQ_ETIMEDOUT; the flag is cleared.
+// (bounded wait) fails the call with IQ_ETIMEDOUT, likewise attention over a
+// paged cache; the flags are cleared.
 int check_device_waits(iq_state* s) {
-  if (s->h_result[5]) {
-    const int f = s->h_result[5];
-    s->h_result[5] = 0;
-    IQ_CUDA(cudaMemset(s->kv_flag.p, 0, sizeof(int)));
-    IQ_CHECK(!(f & kKvTimeout), IQ_ETIMEDOUT,
-             "attention over the cache gave up a bounded device wait; results of this pass are invalid");
-    IQ_CHECK(!f, IQ_ESTATE, "a row stood outside the state's cache");
-  }
-  if (!s->h_result[4]) return IQ_OK;
-  s->h_result[4] = 0;
-  if (int* f = qmv_timeout_flag()) IQ_CUDA(cudaMemset(f, 0, sizeof(int)));
-  set_error("a GEMV gave up waiting for its weight tiles (bounded device wait); results of this pass are invalid");
-  return IQ_ETIMEDOUT;
+  const int gemv = s->h_result[4], kv = s->h_result[5];
+  if (!gemv && !kv) return IQ_OK;
+  s->h_result[4] = s->h_result[5] = 0;
+  if (kv) IQ_CUDA(cudaMemset(s->kv_flag.p, 0, sizeof(int)));
+  if (gemv)
+    if (int* f = qmv_timeout_flag()) IQ_CUDA(cudaMemset(f, 0, sizeof(int)));
+  IQ_CHECK(!gemv, IQ_ETIMEDOUT,
+           "a GEMV gave up waiting for its weight tiles (bounded device wait); results of this pass are invalid");
+  IQ_CHECK(!(kv & kKvTimeout), IQ_ETIMEDOUT,
+           "attention over the cache gave up a bounded device wait; results of this pass are invalid");
+  IQ_CHECK(!kv, IQ_ESTATE, "a row stood outside the state's cache");
+  return IQ_OK;
+}
+
+// The MTP calls': a failed one leaves the device's MTP position where the
+// host's is, so that the call can be made again.
+int check_mtp_waits(iq_state* s) {
+  const int rc = check_device_waits(s);
+  if (!rc) return IQ_OK;
+  IQ_CUDA(set_int_launch(s->ctrl.as<int>() + 5, (int)s->mtp_position, false, s->st, false));
+  IQ_CUDA(cudaStreamSynchronize(s->st));
+  return rc;
 }
 
 int reset_state(iq_state* s) {
@@ -1436,13 +1455,13 @@ int iq_verify(iq_state* s, const uint32_t* tokens, int rows, iq_verify_result* o
   if (rc) return rc;
   IQ_CUDA(cudaStreamSynchronize(s->st));
   if (s->profiling) collect_marks(s);
-  TRY(check_device_waits(s));
   out->accepted = s->h_result[0];
   out->authoritative = s->h_result[1];
   out->committed = s->h_result[2];
+  // (the device has moved on whatever the rows are worth)
   s->position += out->committed;
   s->can_rollback = false;
-  return IQ_OK;
+  return check_device_waits(s);
 }
 
 // Row r of the MTP inputs takes the target's hidden row of the position
@@ -1493,8 +1512,10 @@ int iq_mtp_sync(iq_state* s, int64_t position, const float* prev_hidden, const u
     int rc = run_captured(s, s->mtp_sync_graphs[k - 1], s->mtp_sync_eager[k - 1], [&] { return run_mtp_block(s, k); });
     if (rc) return rc;
   }
+  TRY(fetch_device_waits(s));
   IQ_CUDA(cudaStreamSynchronize(s->st));
   if (s->profiling) collect_marks(s);
+  TRY(check_mtp_waits(s));
   s->mtp_position = position + rows;
   return IQ_OK;
 }
@@ -1530,8 +1551,10 @@ int iq_mtp_draft(iq_state* s, uint32_t seed, const float* hidden, int depth, int
   if (rc) return rc;
   float* ho = s->h_mtp + (int64_t)kMaxK * H;
   IQ_CUDA(cudaMemcpyAsync(ho, s->mtp_out.p, 3 * kMaxDraft * 4, cudaMemcpyDeviceToHost, s->st));
+  TRY(fetch_device_waits(s));
   IQ_CUDA(cudaStreamSynchronize(s->st));
   if (s->profiling) collect_marks(s);
+  TRY(check_mtp_waits(s));
   s->mtp_position += depth;
   const int* ot = reinterpret_cast<const int*>(ho);
   int m = 0;

@@ -50,7 +50,7 @@ struct iq_state {
   // control words: [0]=pos [1]=DeltaNet conv ring index [2..4]=result
   // [5]=MTP pos [6]=DeltaNet update records still to replay (pending)
   iq::DevBuf ctrl;
-  int* h_result = nullptr;   // pinned [4]
+  int* h_result = nullptr;   // pinned: accepted, authoritative, committed, -, GEMV and KV status
   int32_t* h_tokens = nullptr;  // pinned [8]
   iq::DevBuf tokens;
   // DeltaNet
