@@ -61,6 +61,8 @@ struct KvAttnArgs {
   int tq;              // query rows a tile: 8, 16, 32, 64 or the tensor-core kernel's 128
   int slots;           // splits that a tile of query rows can need
   bool narrow;         // never the tensor-core kernel (its rows' results depend on the launch)
+  int wait_limit;      // tries of a device wait, up to 2 us each (kv_attend_launch sets it)
+  bool test_skip;      // tests only: the first CTA's first copy is not requested
   float* part;         // slots > 1: [row][head][slot][hd] unnormalised outputs
   float2* ml;          //            [row][head][slot] {maximum, sum}, base-2 exponents
 };

@@ -35,6 +35,7 @@
 // takes 11 us: start, one pass of loads, and the join, each bound by latency.
 #include <cfloat>
 #include <climits>
+#include <cstdlib>
 #include <type_traits>
 #include "kv_device.cuh"
 #include "kv_split.cuh"
@@ -49,7 +50,6 @@ using namespace kvp;
 constexpr int kTile = kKvTile;
 constexpr int kWarps = 4;
 constexpr int kWaitLimit = 1 << 19;   // of 2 us each: a second
-constexpr int kDrainLimit = 1 << 21;  // for copies already in flight: none may outlive the CTA
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(160, kMinCtas<HD, FMT, NT, F32Q>) kv_attend_ke
     bool ok = true;
     for (int ti = sp.first; ti < sp.end; it++) {
       const int s = it % ST;
-      if (it >= ST && !__all_sync(0xffffffffu, bar_wait(&empty[s], ((it / ST) + 1) & 1, kWaitLimit))) {
+      if (it >= ST && !__all_sync(0xffffffffu, bar_wait(&empty[s], ((it / ST) + 1) & 1, a.wait_limit))) {
         ok = false;
         break;
       }
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(160, kMinCtas<HD, FMT, NT, F32Q>) kv_attend_ke
       for (int c0 = 0; c0 < copies; c0 += 32) {
         const int c = c0 + lane, run = min(c / per, runs - 1), what = c % per;
         const int64_t at = (int64_t)__shfl_sync(0xffffffffu, page, run) * p.nkv + kvh;
-        if (c >= copies) continue;
+        if (c >= copies || (a.test_skip && blockIdx.x == 0 && it == 0 && c == 0)) continue;
         if (what < 2 * kParts) {
           const int part = what % kParts, isv = what / kParts;
           const uint8_t* src = (isv ? p.v : p.k) + at * hb;
@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(160, kMinCtas<HD, FMT, NT, F32Q>) kv_attend_ke
     if (!ok && lane == 0) atomicOr(p.flag, kKvTimeout);
     // no copy outlives the CTA, also when the readers gave up
     for (int s = 0; s < ST; s++)
-      if (it > s) bar_wait(&full[s], ((it - 1 - s) / ST) & 1, kDrainLimit);
+      if (it > s) bar_wait(&full[s], ((it - 1 - s) / ST) & 1, 4 * a.wait_limit);
     return;
   }
 
@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(160, kMinCtas<HD, FMT, NT, F32Q>) kv_attend_ke
     const int s = it % ST, t0 = ti * kTile;
     const uint32_t kt = su32(smem + s * 2 * G_::kTileBytes), vt = kt + G_::kTileBytes;
     const float* sc = scales + s * 128;
-    const bool ok = __all_sync(0xffffffffu, bar_wait(&full[s], (it / ST) & 1, kWaitLimit));
+    const bool ok = __all_sync(0xffffffffu, bar_wait(&full[s], (it / ST) & 1, a.wait_limit));
     float sa[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; n++) sa[n][0] = sa[n][1] = sa[n][2] = sa[n][3] = 0.f;
@@ -765,7 +765,12 @@ void kv_attend_bind(KvAttnArgs& a, void* workspace) {
   a.ml = reinterpret_cast<float2*>(a.part + (int64_t)a.b.rows * a.heads * a.slots * a.pool.hd);
 }
 
-cudaError_t kv_attend_launch(const KvAttnArgs& a, cudaStream_t st) {
+cudaError_t kv_attend_launch(const KvAttnArgs& args, cudaStream_t st) {
+  KvAttnArgs a = args;
+  // tests only, looked up at every launch: a copy that never comes, and waits of
+  // a millisecond for it (every copy that is requested lands long before)
+  a.test_skip = getenv("IQ_KV_TEST_TIMEOUT") != nullptr;
+  a.wait_limit = a.test_skip ? 1 << 9 : kWaitLimit;
   const int tq = a.tq;
   const int64_t ctas = kv_tiles_bound(a, tq) * a.pool.nkv * a.slots;
   if (ctas >= (1ll << 31)) return cudaErrorInvalidValue;

@@ -67,8 +67,6 @@ namespace {
 using namespace kvp;
 
 constexpr int kM = 128, kT = 64;
-constexpr int kWaitLimit = 1 << 19;  // of 2 us each: a second
-constexpr int kDrainLimit = 1 << 21;
 constexpr int kScaleRing = 4;
 constexpr int kSoftWarps = 16, kMmaWarp = 16, kLoadWarp = 17, kExpandWarp = 21;
 
@@ -310,7 +308,7 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
   };
   // a warp's wait: one outcome for all lanes
   auto wait = [&](uint64_t* b, uint32_t parity) {
-    for (int i = 0; i < kWaitLimit; i++) {
+    for (int i = 0; i < a.wait_limit; i++) {
       if (__all_sync(0xffffffffu, bar_try(b, parity))) return true;
       if ((i & 31) == 31 && __any_sync(0xffffffffu, *abort_v)) return false;
     }
@@ -697,7 +695,7 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
     }
     if (leader) commit(&drained);  // every product issued above has completed when this fires
     __syncwarp();
-    bar_wait(&drained, 0, kDrainLimit);
+    bar_wait(&drained, 0, 4 * a.wait_limit);
   } else if (warp < kExpandWarp) {
     // ----------------------------------------------------- bulk copies
     // A warp takes every other tile of keys or values.  The page ids of its
@@ -745,6 +743,7 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
     auto after = [&](int ti) { return sp.next(sp.next(ti)); };
     int it = turn, ti = turn ? sp.next(sp.first) : sp.first, t1 = after(ti);
     bool ok = true;
+    const bool skip_first = a.test_skip && blockIdx.x == 0 && !isv && turn == 0 && lane == 0;
     int page = page_of(ti, ask(ti)), id1 = ask(t1);
     if (ti < sp.end) load_scales(ti, page);
     if (FMT == kKvF16 && isv && ti < sp.end) ok = wait(&qfull, 0);  // the V ring holds the query rows first
@@ -781,7 +780,7 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
         for (int c0 = 0; c0 < runs * kParts; c0 += 32) {
           const int c = c0 + lane, run = min(c / kParts, runs - 1), part = c % kParts;
           const int64_t at = (int64_t)__shfl_sync(0xffffffffu, page, run) * p.nkv + kvh;
-          if (c < runs * kParts)
+          if (c < runs * kParts && !(skip_first && it + c0 == 0))
             bulk_load(su32(ring + s * TB + (part * kT + run * rt) * 128),
                       pool + at * hb + ((int64_t)part * p.page_tokens + tp) * 128, rt * 128, &full[s]);
         }
@@ -799,7 +798,7 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
           requested = n + 1;
           const int t = q * G_::kStageTokens + min(lane, copies - 1) * ct;
           const int64_t at = (int64_t)__shfl_sync(0xffffffffu, page, t >> rs) * p.nkv + kvh;
-          if (lane < copies)
+          if (lane < copies && !(skip_first && n == 0))
             bulk_load(su32(stages + (isv * NS + s) * SB + lane * ct * HD),
                       pool + at * hb + (int64_t)((ti * kT + t) & (p.page_tokens - 1)) * HD, ct * HD, bar);
           __syncwarp();
