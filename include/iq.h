@@ -425,7 +425,8 @@ int iq_kv_attend(const iq_kv* c, const iq_kv_batch* b, const iq_kv_attn* a, cons
                  void* stream);
 /* Synchronize `stream` and report (once) what calls on this cache met:
  * IQ_EINVAL for a position or page id out of range, IQ_ETIMEDOUT when a
- * bounded device wait gave up. */
+ * bounded device wait gave up (the message then names both, where both were
+ * met).  What calls on other streams meet meanwhile is kept for the next. */
 int iq_kv_status(iq_kv* c, void* stream);
 
 #ifdef __cplusplus

@@ -15,6 +15,7 @@
 // and per token and head one f32 scale each for keys and values,
 // [page][head][token].
 #pragma once
+#include <atomic>
 #include <cstdint>
 #include "api_util.h"
 #include "iq_common.cuh"
@@ -100,4 +101,5 @@ struct iq_kv {
   iq::KvPool pool = {};
   iq::DevBuf k, v, ks, vs, flag;
   int device = 0;
+  std::atomic<uint32_t> status_calls{0};
 };

@@ -249,6 +249,11 @@ __global__ void __launch_bounds__(256, 6) kv_read_kernel(const __grid_constant__
   }
 }
 
+// The flag read and cleared in one step: what another stream records meanwhile
+// stays for the next reader.
+__global__ void kv_take_flag_kernel(int* flag, int* out) { *out = atomicExch(flag, 0); }
+constexpr int kStatusWords = 63;  // behind the flag: one for each of so many iq_kv_status calls at once
+
 // Whether every lane's elements start on a multiple of their own size (16
 // bytes at most): base and strides in bytes.
 bool vector_ok(const KvTensor& t, int item, int hd) {
@@ -308,7 +313,7 @@ int kv_create(int format, int kv_heads, int head_dim, int page_tokens, int64_t p
   const size_t bytes = (size_t)pages * kv_heads * (size_t)kv_head_bytes(format, head_dim, page_tokens);
   const size_t sbytes = (size_t)pages * kv_heads * page_tokens * 4;
   DevBuf* bufs[] = {&c.k, &c.v, &c.ks, &c.vs, &c.flag};
-  const size_t sizes[] = {bytes, bytes, sbytes, sbytes, sizeof(int)};
+  const size_t sizes[] = {bytes, bytes, sbytes, sbytes, (1 + kStatusWords) * sizeof(int)};
   const int n = flag ? 4 : 5;
   for (int i = 0; i < n; i++) {
     const cudaError_t e = bufs[i]->reserve(sizes[i]);
@@ -535,14 +540,18 @@ int iq_kv_status(iq_kv* c, void* stream) {
   OnDevice on(c->device);
   IQ_CUDA(on.err);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  int f = 0;
-  IQ_CUDA(cudaMemcpyAsync(&f, c->pool.flag, sizeof f, cudaMemcpyDeviceToHost, st));
+  int f = 0, *word = c->pool.flag + 1 + c->status_calls.fetch_add(1) % kStatusWords;
+  kv_take_flag_kernel<<<1, 1, 0, st>>>(c->pool.flag, word);
+  IQ_CUDA(cudaGetLastError());
+  IQ_CUDA(cudaMemcpyAsync(&f, word, sizeof f, cudaMemcpyDeviceToHost, st));
   IQ_CUDA(cudaStreamSynchronize(st));
-  if (f) IQ_CUDA(cudaMemsetAsync(c->pool.flag, 0, sizeof f, st));
+  const char* page = f & kKvBadPage
+                         ? "a row or a token stood outside its block table, or the table named a page outside the pool"
+                         : "";
   IQ_CHECK(!(f & kKvTimeout), IQ_ETIMEDOUT,
-           "attention over the cache gave up a bounded device wait; results of that call are invalid");
-  IQ_CHECK(!(f & kKvBadPage), IQ_EINVAL,
-           "a row or a token stood outside its block table, or the table named a page outside the pool");
+           "attention over the cache gave up a bounded device wait; results of that call are invalid%s%s",
+           *page ? "; and " : "", page);
+  IQ_CHECK(!*page, IQ_EINVAL, "%s", page);
   return IQ_OK;
 }
 
