@@ -24,6 +24,8 @@ _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 
 P, I64, I32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
 
+_KEPT = 64  # argument structures that a batch or a cache keeps for calls like earlier ones
+
 
 class _Batch(ctypes.Structure):
     _fields_ = [("table", P), ("position", P), ("row_start", P), ("table_ld", I64), ("table_cols", ctypes.c_int32),
@@ -96,6 +98,8 @@ class KvBatch:
         if got is None:
             c = self._c
             got = _Batch(c.table, c.position, c.row_start, c.table_ld, c.table_cols, c.seqs, rows, c.max_rows)
+            if len(self._of_rows) >= _KEPT:
+                self._of_rows.clear()
             self._of_rows[rows] = got
         return got
 
@@ -191,6 +195,8 @@ class KvCache:
         key = q.dtype, heads, scale, window, sinks, chunk
         at = self._attn.get(key)
         if at is None:
+            if len(self._attn) >= _KEPT:
+                self._attn.clear()
             at = self._attn[key] = _Attn(_TYPES[q.dtype], heads, scale, window, sinks, chunk)
         c, need = batch._with(rows), ctypes.c_size_t()
         _lib.check(self._lib.iq_kv_attend_workspace(self._h, c, at, need))
