@@ -8,7 +8,8 @@
     k, v = cache.read(batch, dtype=torch.float32, rows=8)
 
 One ``KvCache`` holds one layer.  Calls are enqueued on the current stream of
-the cache's device unless ``stream`` is given.
+the cache's device unless ``stream`` (a handle) is given; the tensors of such a
+call may be let go at once.
 """
 from __future__ import annotations
 
@@ -141,6 +142,17 @@ class KvCache:
             x.record_stream(torch.cuda.current_stream(self.device))
         return x
 
+    def _on(self, stream, batch, *tensors):
+        """The stream for a call on ``tensors``; one given by handle reads (or
+        writes) them and the batch after the caller may have let them go."""
+        if stream is None:
+            return self._stream(None)
+        st = torch.cuda.ExternalStream(stream, device=self.device)
+        for x in (*tensors, *batch._keep):
+            if x is not None and x.numel():
+                x.record_stream(st)
+        return stream
+
     def _rows(self, name, x, heads, batch):
         shape = x.shape
         if x.dtype not in _TYPES:
@@ -159,7 +171,8 @@ class KvCache:
         if k.shape != v.shape or k.dtype != v.dtype:
             raise ValueError("keys and values must have one shape and type")
         a, b = self._rows("keys", k, self.kv_heads, batch), self._rows("values", v, self.kv_heads, batch)
-        _lib.check(self._lib.iq_kv_append(self._h, batch._with(k.shape[0]), _TYPES[k.dtype], *a, *b, self._stream(stream)))
+        _lib.check(self._lib.iq_kv_append(self._h, batch._with(k.shape[0]), _TYPES[k.dtype], *a, *b,
+                                          self._on(stream, batch, k, v)))
 
     def read(self, batch: KvBatch, *, rows: int, dtype=torch.float32, out=None, stream=None):
         """(keys, values) that the cache holds at the batch's ``rows`` rows;
@@ -175,7 +188,8 @@ class KvCache:
         if k.shape != v.shape or k.dtype != v.dtype or k.shape[0] != rows:
             raise ValueError("keys and values must have one shape and type, and the batch's rows")
         a, b = self._rows("keys", k, self.kv_heads, batch), self._rows("values", v, self.kv_heads, batch)
-        _lib.check(self._lib.iq_kv_read(self._h, batch._with(rows), _TYPES[k.dtype], *a, *b, self._stream(stream)))
+        _lib.check(self._lib.iq_kv_read(self._h, batch._with(rows), _TYPES[k.dtype], *a, *b,
+                                        self._on(stream, batch, k, v)))
         return k, v
 
     def attend(self, q: torch.Tensor, batch: KvBatch, *, scale: float = 0.0, window: int = 0, sinks: int = 0,
@@ -204,7 +218,7 @@ class KvCache:
         if n:
             ws = q.new_empty(n, dtype=torch.uint8) if stream is None else self._new(n, torch.uint8, stream)
         _lib.check(self._lib.iq_kv_attend(self._h, c, at, *a, *b, None if ws is None else ws.data_ptr(), n,
-                                          self._stream(stream)))
+                                          self._on(stream, batch, q, out)))
         return out
 
     def status(self, stream=None) -> None:

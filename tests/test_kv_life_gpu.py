@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from inferq_b200.kv import KvBatch
 from test_kv_gpu import Sequences, close
 
 pytestmark = pytest.mark.gpu
@@ -17,4 +18,34 @@ def test_calls_of_ever_new_arguments_keep_no_more_and_more(cuda):
         s.cache.read(whole, rows=i)
     assert len(s.cache._attn) <= 64 and len(b._of_rows) <= 64 and len(whole._of_rows) <= 64
     close(s.cache.attend(q, b, scale=0.1), *s.want(scale=0.1), s.dt)
+    s.cache.status()
+
+
+def test_a_call_on_a_stream_given_by_handle_holds_its_tensors(cuda):
+    """Keys, queries and the batch are let go while the stream is still busy with earlier work, and their memory is
+    asked for again."""
+    s = Sequences([(300, 0)], heads=8, hd=64, kv_heads=1)
+    k, v = s.cache.read(s.all, rows=300)
+    want = s.cache.attend(s.q.cuda(), s.batch())
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        s.cache.append(torch.zeros_like(k), torch.zeros_like(v), s.all)
+        out = torch.empty_like(want)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)
+        q, table, position = s.q.cuda(), s.table.clone(), s.position.clone()
+        a, b = k.clone(), v.clone()
+        torch.cuda.current_stream().synchronize()
+        s.cache.append(a, b, KvBatch(table, position), stream=side.cuda_stream)
+        s.cache.attend(q, KvBatch(table, position), out=out, stream=side.cuda_stream)
+        shapes = [x.shape for x in (q, a, b, table, position)]
+        types = [x.dtype for x in (q, a, b, table, position)]
+        del q, a, b, table, position
+        for _ in range(3):
+            again = [torch.full(shape, 1, dtype=dt, device="cuda") for shape, dt in zip(shapes, types)]
+        torch.cuda.synchronize()
+        del again
+        assert torch.equal(s.cache.read(s.all, rows=300)[0], k)
+        assert torch.equal(out, want)
     s.cache.status()
