@@ -14,6 +14,7 @@ call may be let go at once.
 from __future__ import annotations
 
 import ctypes
+import sys
 
 import torch
 
@@ -103,6 +104,17 @@ class KvBatch:
                 self._of_rows.clear()
             self._of_rows[rows] = got
         return got
+
+
+# Caches let go of while the current stream was captured, freed with the next one.
+_dropped: list[tuple] = []
+
+
+def _free_dropped():
+    while _dropped:
+        device, h = _dropped.pop()
+        torch.cuda.synchronize(device)
+        _lib._lib.iq_kv_destroy(h)
 
 
 class KvCache:
@@ -228,7 +240,9 @@ class KvCache:
 
     def __del__(self):
         h = getattr(self, "_h", None)
-        if h is not None and _lib is not None and _lib._lib is not None:
-            torch.cuda.synchronize(self.device)
-            _lib._lib.iq_kv_destroy(h)
-            self._h = None
+        if h is None or sys is None or sys.is_finalizing():  # (the process's end frees it)
+            return
+        self._h = None
+        _dropped.append((self.device, h))
+        if not torch.cuda.is_current_stream_capturing():  # neither waiting nor freeing may be captured: later then
+            _free_dropped()

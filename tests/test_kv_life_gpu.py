@@ -1,8 +1,12 @@
 """What a cache and a batch keep, and for how long."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
-from inferq_b200.kv import KvBatch
+from inferq_b200.kv import KvBatch, KvCache
 from test_kv_gpu import Sequences, close
 
 pytestmark = pytest.mark.gpu
@@ -49,3 +53,38 @@ def test_a_call_on_a_stream_given_by_handle_holds_its_tensors(cuda):
         assert torch.equal(s.cache.read(s.all, rows=300)[0], k)
         assert torch.equal(out, want)
     s.cache.status()
+
+
+def test_a_cache_let_go_under_capture_is_freed_later(cuda):
+    s, lone = Sequences([(2, 60)], heads=8, hd=64, kv_heads=1), KvCache(1, 64, 1000)
+    q, b = s.q.cuda(), s.batch()
+    want = s.cache.attend(q, b)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        del lone
+        out = s.cache.attend(q, b)
+    graph.replay()
+    assert torch.equal(out, want)
+    free = torch.cuda.mem_get_info()[0]
+    del graph, out
+    KvCache(1, 64, 1)
+    assert torch.cuda.mem_get_info()[0] >= free + 1000 * 64 * 64 * 2
+    s.cache.status()
+
+
+CHILD = r"""
+import builtins
+import sys
+import torch
+from inferq_b200.kv import KvCache
+cache, builtins.kept, sys.kept = (KvCache(1, 64, 4) for _ in range(3))
+cache.cycle = cache, torch
+print(cache.nbytes)
+"""
+
+
+def test_a_cache_may_outlive_the_program(cuda):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", CHILD], capture_output=True, text=True, timeout=300, cwd=root)
+    assert r.returncode == 0 and not r.stderr, r.stderr
