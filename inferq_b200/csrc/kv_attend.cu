@@ -530,8 +530,9 @@ __global__ void __launch_bounds__(160, kMinCtas<HD, FMT, NT, F32Q>) kv_attend_ke
       for (int b = 0; b < kMine; b++) {
         const int blk = warp * kMine + b;
         // i8: elements 4g .. 4g+3 of the block; f16: g, g+8, g+16, g+24
-        const float x[4] = {o[b][0][n][e] * back * f, o[b][0][n][2 + e] * back * f, o[b][1][n][e] * back * f,
-                            o[b][1][n][2 + e] * back * f};
+        // (back last: before the division by the sum a value near f32's end would pass it)
+        const float x[4] = {o[b][0][n][e] * f * back, o[b][0][n][2 + e] * f * back, o[b][1][n][e] * f * back,
+                            o[b][1][n][2 + e] * f * back};
         auto put = [&](auto* dst, bool v4) {
           using T = std::remove_reference_t<decltype(*dst)>;
           if constexpr (FMT == kKvI8) {
