@@ -68,6 +68,11 @@ using namespace kvp;
 
 constexpr int kM = 128, kT = 64;
 constexpr int kScaleRing = 4;
+// Keys' scales are taken times 2^-14 and the queries' factors times 2^14: scores
+// of keys up to 2^118 stay below f32's end until a small query brings them back.
+// i8 values' scales, 2^8 above f16's for the same values, are taken times 2^-8:
+// p = 2^(4 - ev) then stays 20 binades above f32's beginning for values of 2^119.
+constexpr float kKeyDown = 0x1p-14f, kKeyUp = 0x1p14f;
 constexpr int kSoftWarps = 16, kMmaWarp = 16, kLoadWarp = 17, kExpandWarp = 21;
 
 template <int HD, int FMT, bool F32Q>
@@ -376,7 +381,8 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
             *reinterpret_cast<uint32_t*>(d) = *reinterpret_cast<const uint32_t*>(hi);
             if constexpr (F32Q) *reinterpret_cast<uint32_t*>(dl) = *reinterpret_cast<const uint32_t*>(lo);
           }
-          if (lane == 0) tops[row] = fmaxf(pow2i(e) * fabsf(a.scale_log2e), FLT_MIN);  // never 0: hidden scores stay -inf
+          // (never 0 or infinite: hidden scores stay -inf, others finite)
+          if (lane == 0) tops[row] = fminf(fmaxf(pow2i(e) * fabsf(a.scale_log2e) * kKeyUp, FLT_MIN), FLT_MAX);
         }
       }
     }
@@ -586,7 +592,8 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
       const float l = (tops[row] + tops[kM + row]) + (sums[row] + sums[kM + row]);
       const int grow = tr.row0 + rr / group, h = kvh * group + rr % group;
       const int64_t rh = (int64_t)grow * a.heads + h;
-      const float f = a.slots > 1 ? 1.f : l != 0.f ? __fdiv_rn(1.f, l) : 0.f;
+      constexpr float kUp = FMT == kKvI8 ? 0x1p8f : 1.f;
+      const float f = a.slots > 1 ? kUp : l != 0.f ? __fdiv_rn(kUp, l) : 0.f;
       if (a.slots > 1 && live && part == 0) a.ml[rh * a.slots + slot] = make_float2(m - 7.f + (float)ev, l);
       // A row's elements lie with one thread: they go to shared memory, a row
       // of hd elements and 16 bytes apart (so that eight lanes' stores meet
@@ -757,8 +764,9 @@ __global__ void __launch_bounds__(Geo<HD, FMT, F32Q>::kThreads, 1)
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         const int t = lane + 32 * h;
-        sc[isv * kT + t] = sv[h];
-        const uint32_t bits = __float_as_uint(sv[h]);
+        const float s = sv[h] * (!isv ? kKeyDown : FMT == kKvI8 ? 0x1p-8f : 1.f);
+        sc[isv * kT + t] = s;
+        const uint32_t bits = __float_as_uint(s);
         if (bits < 0x7f800000u && ti * kT + t < sp.tokens) top = max(top, bits);
       }
       top = __reduce_max_sync(0xffffffffu, top);

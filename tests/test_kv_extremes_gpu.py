@@ -1,5 +1,5 @@
-"""Attention over values near the ends of f32's range, whose
-results are ordinary numbers: against the definition in 64 bits,
+"""Attention over keys, values and queries near the ends of f32's range, whose
+scores and results are ordinary numbers: against the definition in 64 bits,
 with the tolerances of test_kv_gpu."""
 import pytest
 import torch
@@ -16,7 +16,16 @@ def run(s, **kw):
     return got, want, most
 
 
-@pytest.mark.parametrize("rows,chunk", [(1, 0), (1, 128), (8, 128)])
+@pytest.mark.parametrize("rows,chunk", [(1, 0), (1, 128), (3, 0), (8, 128), (70, 0), (70, 640)])
+@pytest.mark.parametrize("fmt,dtype", [("i8", "f32"), ("f16", "f32"), ("i8", "bf16"), ("f16", "bf16")])
+@pytest.mark.parametrize("binades", [100, 110, 118, -90, -100])
+def test_keys_and_queries(cuda, binades, fmt, dtype, rows, chunk):
+    s = Sequences([(rows, 333)], heads=8, kv_heads=1, hd=64, fmt=fmt, dtype=dtype)
+    s.k, s.q = s.k * 2.0 ** binades, s.q * 2.0 ** -binades
+    close(*run(s, chunk=chunk), s.dt)
+
+
+@pytest.mark.parametrize("rows,chunk", [(1, 0), (1, 128), (3, 0), (8, 128), (70, 0), (70, 640)])
 @pytest.mark.parametrize("fmt,dtype", [("i8", "f32"), ("f16", "f32"), ("i8", "bf16"), ("f16", "bf16")])
 @pytest.mark.parametrize("binades", [100, 110, 116, -80, -90])
 def test_values(cuda, binades, fmt, dtype, rows, chunk):
@@ -27,7 +36,7 @@ def test_values(cuda, binades, fmt, dtype, rows, chunk):
 
 
 @pytest.mark.parametrize("fmt", ["i8", "f16"])
-@pytest.mark.parametrize("rows,chunk", [(1, 0), (8, 128)])
+@pytest.mark.parametrize("rows,chunk", [(1, 0), (8, 128), (70, 0)])
 def test_many_small_weights_under_huge_values(cuda, fmt, rows, chunk):
     """One token 14 nats above thousands of others that together weigh as much as some thousandths of it."""
     s = Sequences([(rows, 5000)], heads=8, kv_heads=1, hd=64, fmt=fmt)
