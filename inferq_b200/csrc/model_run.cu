@@ -586,21 +586,35 @@ int state_kv_attention(iq_state* s, int fi, const int* pos, int rows, const floa
   ++s->launch_count;
   IQ_CUDA(kv_append_launch(a.pool, a.b, F32, KvTensor{const_cast<float*>(k), kvd, hd},
                            KvTensor{const_cast<float*>(v), kvd, hd}, s->st));
-  a.q = KvTensor{const_cast<float*>(q), nhd, hd};
-  a.out = KvTensor{out, nhd, hd};
   a.dtype = F32;
   a.heads = c.num_attention_heads;
   a.scale_log2e = (float)(1.4426950408889634 / sqrt((double)hd));
-  a.window = s->kv_window;
-  a.sinks = s->kv_window ? s->kv_sinks : 0;
-  a.chunk = narrow ? kStateChunk : 0;
   a.narrow = narrow;
-  const size_t need = kv_attend_plan(a, rows);
-  if (grow) IQ_CUDA(ws.reserve(need));
-  IQ_CHECK(ws.bytes >= need, IQ_ESTATE, "attention workspace of %zu bytes, %zu are needed", ws.bytes, need);
-  kv_attend_bind(a, ws.p);
-  s->launch_count += a.slots > 1 ? 2 : 1;
-  IQ_CUDA(kv_attend_launch(a, s->st));
+  // rows r0 .. r0 + n - 1; the bytes that they need
+  auto plan = [&](int r0, int n) {
+    a.q = KvTensor{const_cast<float*>(q) + r0 * nhd, nhd, hd};
+    a.out = KvTensor{out + r0 * nhd, nhd, hd};
+    a.b.position = pos + r0 / 8;
+    a.b.rows = n;
+    if (!narrow) a.b.table_cols = (int)ceil_div(s->position + r0 + n, kStatePage);
+    a.window = s->kv_window;
+    a.sinks = s->kv_window ? s->kv_sinks : 0;
+    a.chunk = narrow ? kStateChunk : 0;
+    return kv_attend_plan(a, n);
+  };
+  // Far into a sequence a pass of 512 rows would leave gigabytes of partial
+  // results (one of hd + 2 floats a row, head and 640 tokens): fewer rows at once.
+  constexpr size_t kMostWorkspace = (size_t)512 << 20;
+  int step = rows;
+  while (!narrow && step > 64 && plan(0, step) > kMostWorkspace) step = (int)align_up(step / 2, 8);
+  for (int r0 = 0; r0 < rows; r0 += step) {
+    const size_t need = plan(r0, std::min(step, rows - r0));
+    if (grow) IQ_CUDA(ws.reserve(need));
+    IQ_CHECK(ws.bytes >= need, IQ_ESTATE, "attention workspace of %zu bytes, %zu are needed", ws.bytes, need);
+    kv_attend_bind(a, ws.p);
+    s->launch_count += a.slots > 1 ? 2 : 1;
+    IQ_CUDA(kv_attend_launch(a, s->st));
+  }
   return IQ_OK;
 }
 

@@ -126,8 +126,9 @@ struct iq_state {
 
 
 namespace iq {
-// Rows of layer fi's paged cache at *pos, *pos + 1, .. (device): written from
-// k, v [rows][kv_head][hd] f32 and attended to by q [rows][head][hd] f32.
+// Rows of layer fi's paged cache at *pos, *pos + 1, .. (device; where not
+// `narrow`, pos[j] is the position of row 8 j): written from k, v
+// [rows][kv_head][hd] f32 and attended to by q [rows][head][hd] f32.
 // `ws` grows as needed where `grow` is set (never under capture).
 int state_kv_attention(iq_state* s, int fi, const int* pos, int rows, const float* k, const float* v, const float* q,
                        float* out, bool narrow, DevBuf& ws, bool grow);
