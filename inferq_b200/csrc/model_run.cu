@@ -609,7 +609,8 @@ int state_kv_attention(iq_state* s, int fi, const int* pos, int rows, const floa
   while (!narrow && step > 64 && plan(0, step) > kMostWorkspace) step = (int)align_up(step / 2, 8);
   for (int r0 = 0; r0 < rows; r0 += step) {
     const size_t need = plan(r0, std::min(step, rows - r0));
-    if (grow) IQ_CUDA(ws.reserve(need));
+    // (by halves: it needs a little more at every pass, and growing waits for the device)
+    if (grow && ws.bytes < need) IQ_CUDA(ws.reserve(std::max(need, std::min(need + need / 2, kMostWorkspace))));
     IQ_CHECK(ws.bytes >= need, IQ_ESTATE, "attention workspace of %zu bytes, %zu are needed", ws.bytes, need);
     kv_attend_bind(a, ws.p);
     s->launch_count += a.slots > 1 ? 2 : 1;
