@@ -106,14 +106,18 @@ class KvBatch:
         return got
 
 
-# Caches let go of while the current stream was captured, freed with the next one.
+# Caches let go of while a stream was captured, freed when the next is made or let go.
 _dropped: list[tuple] = []
 
 
 def _free_dropped():
     while _dropped:
         device, h = _dropped.pop()
-        torch.cuda.synchronize(device)
+        try:
+            torch.cuda.synchronize(device)
+        except RuntimeError:  # (another thread captures)
+            _dropped.append((device, h))
+            return
         _lib._lib.iq_kv_destroy(h)
 
 
@@ -127,6 +131,7 @@ class KvCache:
         self.kv_heads, self.head_dim, self.pages, self.page_tokens = kv_heads, head_dim, pages, page_tokens
         self.format = format
         self._lib = _lib_()
+        _free_dropped()
         h = P()
         dev = torch.device("cuda" if device is None else device)
         with torch.cuda.device(dev):
