@@ -274,10 +274,10 @@ __global__ void __launch_bounds__(160, kMinCtas<HD, FMT, NT, F32Q>) kv_attend_ke
 #pragma unroll
   for (int n = 0; n < NT; n++) mrow[n][0] = mrow[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.f;
   // Rows have one exponent, evu, until a masked tile: then each has its own,
-  // kept by thread r for row r and at most evu, until a whole tile reaches evu.
+  // which esc keeps as 2^(14 - e), at most evu, until a whole tile reaches evu.
   // (Every row's in every thread's registers: spills, and 25% more time for 64
   // f32 rows of hd 256.)
-  int evu = -100, mine = -100;  // so that 2^(14 - e) is finite
+  int evu = -100;  // so that 2^(14 - e) is finite
   bool one = true;
   bool failed = false;
 
@@ -393,9 +393,9 @@ __global__ void __launch_bounds__(160, kMinCtas<HD, FMT, NT, F32Q>) kv_attend_ke
     float shrink = 0.f, up = 0.f;  // of all rows
     if (own) {
       if (threadIdx.x < TQ) {
-        const int r = threadIdx.x, from = one ? evu : mine;
-        mine = max(from, whole ? evt : max(max(evr[r], evr[TQ + r]), max(evr[2 * TQ + r], evr[3 * TQ + r])));
-        esc[r] = make_float2(shrink_of(from, mine), pow2i(14 - mine));
+        const int r = threadIdx.x, from = one ? evu : 14 - ((__float_as_int(esc[r].y) >> 23) - 127);
+        const int to = max(from, whole ? evt : max(max(evr[r], evr[TQ + r]), max(evr[2 * TQ + r], evr[3 * TQ + r])));
+        esc[r] = make_float2(shrink_of(from, to), pow2i(14 - to));
       }
       consumers_sync();
       one = whole && evt >= evu;
@@ -501,7 +501,7 @@ __global__ void __launch_bounds__(160, kMinCtas<HD, FMT, NT, F32Q>) kv_attend_ke
   }
   // ------------------------------------------------------------- results
   consumers_sync();  // mx and esc are read no more
-  if (threadIdx.x < TQ) esc[threadIdx.x].x = pow2i(one ? evu : mine);
+  if (threadIdx.x < TQ) esc[threadIdx.x].x = one ? pow2i(evu) : __fdiv_rn(16384.f, esc[threadIdx.x].y);
 #pragma unroll
   for (int n = 0; n < NT; n++)
 #pragma unroll
