@@ -25,6 +25,14 @@ class IqError(RuntimeError):
         self.code = code
 
 
+def fits(bits: int = 32, **values: int) -> None:
+    """Raise where a value leaves the signed integer of ``bits`` that the C ABI
+    takes it in (ctypes would pass its low bits)."""
+    for name, v in values.items():
+        if not -(1 << (bits - 1)) <= v < 1 << (bits - 1):
+            raise ValueError(f"{name} of {v} is out of range")
+
+
 def lib() -> ctypes.CDLL:
     global _lib
     if _lib is None:

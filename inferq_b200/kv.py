@@ -87,6 +87,7 @@ class KvBatch:
             raise ValueError(f"row_start has {row_start.shape[0]} entries for {seqs} sequences")
         if max_rows < 0:
             raise ValueError("max_rows cannot be negative")
+        _lib.fits(max_rows=max_rows)
         self.device, self.index = table.device, table.get_device()
         self.seqs = seqs
         self._keep = table, position, row_start
@@ -128,6 +129,8 @@ class KvCache:
                  device=None):
         if format not in FORMATS:
             raise ValueError(f"cache format {format!r}; expected one of {sorted(FORMATS)}")
+        _lib.fits(kv_heads=kv_heads, head_dim=head_dim, page_tokens=page_tokens)
+        _lib.fits(64, pages=pages)
         self.kv_heads, self.head_dim, self.pages, self.page_tokens = kv_heads, head_dim, pages, page_tokens
         self.format = format
         self._lib = _lib_()
@@ -226,6 +229,7 @@ class KvCache:
         key = q.dtype, heads, scale, window, sinks, chunk
         at = self._attn.get(key)
         if at is None:
+            _lib.fits(window=window, sinks=sinks, chunk=chunk)
             if len(self._attn) >= _KEPT:
                 self._attn.clear()
             at = self._attn[key] = _Attn(_TYPES[q.dtype], heads, scale, window, sinks, chunk)

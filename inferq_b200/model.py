@@ -146,6 +146,8 @@ class State:
     def __init__(self, model: Model, max_positions: int, *, kv: str = "f32", window: int = 0, sinks: int = 0):
         if kv not in self.KV_FORMATS:
             raise ValueError(f"KV cache format {kv!r}; expected one of {sorted(self.KV_FORMATS)}")
+        _lib.fits(window=window, sinks=sinks)
+        _lib.fits(64, max_positions=max_positions)
         self.model = model
         h = P()
         _lib.check(lib().iq_state_create_kv(model._h, max_positions, self.KV_FORMATS[kv], window, sinks, ctypes.byref(h)))
