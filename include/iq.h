@@ -418,7 +418,10 @@ typedef struct iq_kv_attn {
   int32_t chunk;
 } iq_kv_attn;
 /* Bytes of device workspace that iq_kv_attend needs for such a batch (its
- * host fields only are read); 16-byte aligned, one for each call in flight. */
+ * host fields only are read); 16-byte aligned, one for each call in flight.
+ * head_dim + 2 floats a row, head and split, so that f32 rows above 64 query
+ * rows (a split is at most 640 tokens) over a long table need much: 512 rows of
+ * 16 heads of 256 over 131072 tokens 1.7 GB; fewer rows a call need less. */
 int iq_kv_attend_workspace(const iq_kv* c, const iq_kv_batch* b, const iq_kv_attn* a, size_t* bytes);
 int iq_kv_attend(const iq_kv* c, const iq_kv_batch* b, const iq_kv_attn* a, const void* q, int64_t q_row,
                  int64_t q_head, void* out, int64_t out_row, int64_t out_head, void* workspace, size_t workspace_bytes,

@@ -28,11 +28,13 @@
 // and does not depend on NT: a row's result is the same in any batch.
 //
 // Bound: the cache's bytes for 8 query rows (one f16 token over 262144 positions
-// of 2 heads of 256: 86 us, 6.3 TB/s with its join; i8: 54 us, 5.0 TB/s, where
-// the chain of a tile and a CTA's start and end weigh twice as much; 64 bf16
-// tokens over 6000 i8 positions each: 78 us, 5.1 TB/s); the tensor pipe and
-// shared memory from about 64 query rows on.  One token over 4096 positions
-// takes 11 us: start, one pass of loads, and the join, each bound by latency.
+// of 2 heads of 256: 87 us, 6.2 TB/s with its join; bf16 over i8: 54 us, 5.1
+// TB/s, f32 59, where the chain of a tile and a CTA's start and end weigh twice
+// as much; 64 bf16 tokens over 6000 i8 positions each: 79 us, 5.1 TB/s); the
+// tensor pipe and shared memory from about 64 query rows on (spills too: 64 f32
+// rows of hd 256 want some 90 registers more than there are).  One token over
+// 4096 positions takes 9.5 us: start, one pass of loads, and the join, each
+// bound by latency.
 #include <cfloat>
 #include <climits>
 #include <cstdlib>

@@ -15,7 +15,7 @@
 // us instead of 1140).  TMEM: O in hd columns, the buffers of S (64 columns
 // each; P replaces S in place), Q.  Of S there is room for two buffers at hd
 // 256 and four below, where scores then run three tiles ahead of the sums (two
-// and four, hd 128: 1035 and 930 us).  K tiles are K-major and V tiles MN-major
+// and four, hd 128: 1035 and 930 us when measured side by side).  K tiles are K-major and V tiles MN-major
 // in the 128-byte swizzle, in which the f16 cache already keeps its pages: its
 // tiles arrive by bulk copies alone.  i8 tiles arrive as bytes in small stages,
 // and eight warps expand them to f16 integers.
@@ -51,9 +51,9 @@
 // winds down (copies and MMAs drained, TMEM freed) without results.
 //
 // Bound: the chain scores -> softmax -> values of a tile, of which two are in
-// flight (tensor pipe active half of the cycles, issue slots 45%).  2048 bf16
-// rows of 16 heads over 32768 tokens of 2 heads of 256, unsplit: f16 1130 us
-// (942 TFLOP/s, 57% of a measured GEMM's rate), i8 1405 us; hd 128 930 us.
+// flight (tensor pipe active half of the cycles, issue slots 49%).  2048 rows of
+// 16 heads over 32768 tokens of 2 heads of 256: bf16 over f16 1093 us (975
+// TFLOP/s, 58% of a measured GEMM's rate), over i8 1399 us; hd 128 987 and 1124.
 #include <cfloat>
 #include <climits>
 #include <type_traits>

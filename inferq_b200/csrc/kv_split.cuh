@@ -173,10 +173,19 @@ constexpr KvNarrow kv_narrow(int format, int hd, int nt, bool f32) {
 // Query rows of a tile: the fewest of 8, 16, 32, 64 that take a sequence's
 // rows of one KV head at once, or the tensor-core kernel's 128: above 64 rows
 // unless the call keeps to the other, and above 16 where the split is free
-// too (16 sequences over 4127 tokens, 8 heads to a KV head, f32 and bf16 rows:
-// of 2 rows 34 and 29 us with tiles of 16; of 4 rows 78 and 51 us with tiles of
-// 32; of 8 rows 159 and 124 us with tiles of 64; with tiles of 128 55 and 47 us
-// whichever of these).
+// too.  us for f32 and bf16 rows, i8, tiles of 128 and of up to 64 (as few as
+// take a sequence's rows):
+//   8 heads of 256  16 x 4 rows over 4127    69, 57     85, 74
+//                   16 x 8 over 4127         71, 59    180, 161
+//                   16 x 8 over 700          24, 22     42, 36
+//                   1 x 4 over 4096          22, 20     20, 18
+//                   1 x 8 over 32768         33, 28     72, 58
+//   4 of 128        16 x 8 over 4127        159, 104   196, 160
+//                   1 x 8 over 32768         74, 48     83, 70
+//   4 of 64         16 x 8 over 4127         47, 45     50, 47
+//                   64 x 8 over 2000         81, 60     75, 66
+// One short sequence, and many of small heads in f32, would take the smaller
+// tiles by a tenth.
 inline int kv_tile_query_rows(const KvAttnArgs& a, int max_rows) {
   const int64_t r = (int64_t)(max_rows ? std::min(max_rows, a.b.rows) : a.b.rows) * (a.heads / a.pool.nkv);
   if (!a.narrow && r > (a.chunk ? 64 : 16)) return 128;
@@ -221,9 +230,9 @@ inline size_t kv_plan(KvAttnArgs& a, int max_rows) {
     // that for f32 rows) at hd 256, in the tensor-core kernel 1.1 us (1.8).
     // Several sequences are taken to be of mixed lengths, two thirds of the
     // table on average: an SM that got long ones only sets the time (64 bf16
-    // sequences of up to 8209 tokens, i8, hd 256: chunks of 8256 take 136 us,
-    // of 4160 94, of 2048 69, of 1024 78, of 256 91, of 128 116; the rule's
-    // 1408 takes 85, and 64 sequences of 6000 tokens 78 of at best 72).
+    // sequences of up to 8209 tokens, i8, hd 256: chunks of 8256 take 144 us,
+    // of 4160 101, of 2048 70, of 1024 79, of 256 93, of 128 118; the rule's
+    // 1408 takes 87, and 64 sequences of 6000 tokens 79 of at best 72).
     const bool wide = tq == 128, f32 = a.dtype == F32;
     const int elt = a.pool.format == kKvI8 ? 1 : 2;
     const double read = (2.0 * kKvTile * a.pool.hd * elt + 512) / 43.9e3;
