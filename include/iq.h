@@ -399,7 +399,7 @@ int iq_kv_read(const iq_kv* c, const iq_kv_batch* b, int dtype, void* k, int64_t
  * are f32, f32 queries and weights enter the matrix instructions as two f16
  * parts each, others rounded to f16 (a row's queries over a power of two, so
  * that bf16's range is kept).  Keys and values whose largest element lies
- * between 2^-88 and 2^119 keep their accuracy; beyond, results lose bits.
+ * between 2^-88 and 2^118 keep their accuracy; beyond, results lose bits.
  * out may be q itself (with its strides); no other overlap is allowed.
  * chunk: tokens per split of a sequence (a multiple of 64), counted from
  * position 0, whose partial results are joined in order; 0 lets the call

@@ -15,10 +15,10 @@
 // us instead of 1140).  TMEM: O in hd columns, the buffers of S (64 columns
 // each; P replaces S in place), Q.  Of S there is room for two buffers at hd
 // 256 and four below, where scores then run three tiles ahead of the sums (two
-// and four, hd 128: 1035 and 930 us when measured side by side).  K tiles are K-major and V tiles MN-major
-// in the 128-byte swizzle, in which the f16 cache already keeps its pages: its
-// tiles arrive by bulk copies alone.  i8 tiles arrive as bytes in small stages,
-// and eight warps expand them to f16 integers.
+// and four side by side, hd 128: 1035 and 930 us).  K tiles are K-major and V
+// tiles MN-major in the 128-byte swizzle, in which the f16 cache already keeps
+// its pages: its tiles arrive by bulk copies alone.  i8 tiles arrive as bytes in
+// small stages, and eight warps expand them to f16 integers.
 //
 // f32 rows enter as two f16 parts: Q's second part is a shared-memory operand
 // of a second product into the same S, P's second part lies beside the first.
